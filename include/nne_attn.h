@@ -342,6 +342,117 @@ int nne_qkv_rope_ws(const float *x, int64_t x_row_stride, const float *w_packed,
                     int64_t C, int64_t Hq, int64_t Hkv, int64_t d, const nne_workspace_t *ws,
                     void *stream);
 
+/* ---- paged KV cache and drafted tokens -----------------------------------
+ * No counterpart in the reference, whose caches are one tensor per layer
+ * (src/nn/kv_cache.rs:11-74): a serving loop over many sequences keeps their
+ * rows in pages of one pool, and verifies several drafted tokens per step.
+ *
+ * A layer's pool holds n_pages pages of page_size rows for each KV head, K and
+ * V alike: [n_pages][Hkv][page_size][d], contiguous, d a multiple of 8 and at
+ * most 256, any page_size.  Row r of sequence b is row r % page_size of page
+ * table[b * max_pages + r / page_size].  (An nne_kv_append cache is a pool of
+ * B pages of `capacity` rows with table[b] = b.)  Rows are float32, or bfloat16
+ * rounded to nearest once when they are appended; queries, outputs and new rows
+ * are float32, and every sum is too.
+ *
+ * lens[b] rows of sequence b count.  A step puts its new tokens' rows behind
+ * them (nne_paged_append), attends with its queries to the counted rows and
+ * the new ones (nne_paged_attention), in every layer, and then accepts some of
+ * the new rows (nne_paged_commit), which advances lens.  The layers share
+ * table and lens.
+ *
+ * A step's T tokens per sequence form a tree: parents[b * T + t] < t is the
+ * token that t follows, -1 the last counted row.  NULL parents: a chain, each
+ * token following the one before (a decode step is T = 1).  counts[b] <= T of
+ * sequence b's tokens exist (NULL: all T).  depths[b * T + t] is how many of
+ * the step's tokens precede t on its path (NULL: t), so t's position is
+ * lens[b] + depths[b * T + t].
+ *
+ * Arrays come twice where the host validates or sizes a launch with them, as
+ * lens does: *_dev on the device, *_host the same values on the host.  Kernels
+ * take lengths, counts, depths and tables from the device, so a captured graph
+ * replays for whatever these hold at the time, with the launch split that the
+ * captured call chose.  table_host may be NULL: page numbers are then not
+ * checked on the host.  The kernels never leave the pool: a row whose page is
+ * outside [0, n_pages) is not written, and attention leaves it out. */
+enum { NNE_F32 = 0, NNE_BF16 = 1 };
+
+typedef struct nne_paged_cache {
+    void *k, *v;               /* one layer's pools, 16-byte aligned */
+    int64_t dtype;             /* NNE_F32 or NNE_BF16 */
+    int64_t n_pages, Hkv, page_size, d;   /* n_pages * Hkv * page_size < 2^31 */
+    int64_t B, max_pages;      /* sequences, pages a sequence may have */
+    const int32_t *table;      /* device [B][max_pages] */
+    const int32_t *table_host; /* host copy, or NULL */
+    int32_t *lens_dev, *lens_host;        /* [B] */
+} nne_paged_cache_t;
+
+/* Norm of every head of q and k, and rotary embedding, in one pass over them:
+ *   y = x / sqrt(mean(x^2) + eps) * weight,  out = y * cos + rotate_half(y) * sin
+ * (RMSNorm over the d values of a head, then RotaryEmbedding::apply,
+ * llama.rs:110-157).  q and k are [B, H, T, d] views with the same B, T and d;
+ * token t of sequence b is rotated with table row start[b] + t, or with depths
+ * start[b] + depths[b * T + t].  weights are [d], NULL: ones.  NULL cos_table
+ * and sin_table: no rotation, and start may be NULL.  has_norm = 0: y = x, the
+ * rotation alone (no weights then).  NULL k: q alone.
+ * q_out may be q, and k_out k, with the same strides.  d must be even.
+ * NNE_ESHAPE / NNE_EINVAL as nne_rope_apply, and for eps < 0. */
+int nne_qk_norm_rope(const float *q, const int64_t q_shape[4], const int64_t q_strides[4],
+                     float *q_out, const int64_t q_out_strides[4], const float *k,
+                     const int64_t k_shape[4], const int64_t k_strides[4], float *k_out,
+                     const int64_t k_out_strides[4], const float *q_weight, const float *k_weight,
+                     int has_norm, float eps, const float *cos_table, const float *sin_table,
+                     int64_t max_seq_len, int64_t table_head_dim, const int32_t *start_dev,
+                     const int32_t *start_host, const int32_t *depths_dev,
+                     const int32_t *depths_host, void *stream);
+
+/* Writes the rows of T new tokens, k_new / v_new [B, Hkv, T, d] views, behind
+ * the lens[b] rows of every sequence, the keys rotated at their tokens'
+ * positions on the way (as nne_rope_apply rounds it, then to the pool's type;
+ * NULL cos_table and sin_table: as they are).  lens stays: nne_paged_commit
+ * advances it, and until then another call writes the same rows again.
+ * NNE_ECAPACITY (nothing written) if a sequence has no room for its rows in
+ * max_pages pages; with table_host NNE_EINVAL if a row has no page or two
+ * sequences would write one page. */
+int nne_paged_append(const nne_paged_cache_t *cache, const float *k_new,
+                     const int64_t k_new_strides[4], const float *v_new,
+                     const int64_t v_new_strides[4], int64_t T, const int32_t *counts_dev,
+                     const int32_t *counts_host, const int32_t *depths_dev,
+                     const int32_t *depths_host, const float *cos_table, const float *sin_table,
+                     int64_t max_seq_len, int64_t table_head_dim, void *stream);
+
+/* Attention of T appended tokens' queries q [B, Hq, T, d] (Hkv divides Hq;
+ * head mapping and scale as nne_attention_forward): token t of sequence b sees
+ * the lens[b] counted rows, and of the new ones itself and those before it on
+ * its path.  Rows of o for tokens past counts[b] are left as they were.  At
+ * most 256 tokens with parents, any number in a chain.  What a token does not
+ * see has no part in its result, whatever it holds.  ws: at least
+ * nne_paged_workspace_size, or NULL for the library's per-stream one (a stream
+ * under capture must have one that is large enough already: NNE_EINVAL). */
+int nne_paged_attention(const nne_paged_cache_t *cache, const float *q, const int64_t q_strides[4],
+                        float *o, const int64_t o_strides[4], int64_t Hq, int64_t T,
+                        const int32_t *counts_dev, const int32_t *counts_host,
+                        const int32_t *parents_dev, const int32_t *parents_host, int has_scale,
+                        float scale, const nne_workspace_t *ws, void *stream);
+
+/* Workspace of nne_paged_attention with Hq query heads and up to T tokens, for
+ * any lengths, and of nne_paged_commit. */
+int nne_paged_workspace_size(const nne_paged_cache_t *cache, int64_t Hq, int64_t T,
+                             nne_workspace_size_t *out);
+
+/* Accepts counts[b] of sequence b's new rows: those of the tokens paths[b * J]
+ * < paths[b * J + 1] < ... (counts[b] <= J), which become rows lens[b],
+ * lens[b] + 1, ... in each of n_layers layers, and lens[b] += counts[b].
+ * cache's k and v are the first layer's pools; the next layer's lie
+ * layer_stride elements behind.  NULL paths: the first counts[b] tokens as
+ * they lie.  NULL counts_dev: counts_host[0] for every sequence, and the call
+ * needs no device array.  ws as for nne_paged_attention (counters only).
+ * NNE_EINVAL (nothing moved) for paths that do not ascend or leave the pages. */
+int nne_paged_commit(const nne_paged_cache_t *cache, int64_t n_layers, int64_t layer_stride,
+                     const int32_t *counts_dev, const int32_t *counts_host,
+                     const int32_t *paths_dev, const int32_t *paths_host, int64_t J,
+                     const nne_workspace_t *ws, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

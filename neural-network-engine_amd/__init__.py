@@ -19,6 +19,14 @@ engine's attention API (elvin-mark/neural-network-engine):
 * ``MultiHeadAttention`` -- src/nn/attention.rs:9-210 (GPT-2 / Whisper self- and
   cross-attention) and ``WhisperKVCache`` -- src/models/whisper.rs:325-350
 
+and, for serving loops, operators that the reference has no counterpart of:
+
+* ``PagedKVCache`` -- a cache of pages, float32 or bfloat16, with ``append``
+  (rotation on the way), ``attend`` (one new token, a chain, or a ``DraftTree``)
+  and ``commit`` (an accepted path)
+* ``qk_norm_rope`` -- per-head norm of queries and keys and the rotation, in one
+  pass
+
 Tensors are torch tensors on the GPU (torch is used only for device memory and
 streams).  Errors raise the EngineError variant the reference would return.
 There is no CPU path: if the HIP library is missing, importing works but every
@@ -83,6 +91,16 @@ class NneWorkspace(ctypes.Structure):
 class NneWorkspaceSize(ctypes.Structure):
     """nne_workspace_size_t."""
     _fields_ = [("records_bytes", ctypes.c_uint64), ("n_counters", ctypes.c_uint64)]
+
+
+class NnePagedCache(ctypes.Structure):
+    """nne_paged_cache_t: one layer's pools and the sequences' pages."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int64),
+                ("n_pages", ctypes.c_int64), ("Hkv", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("d", ctypes.c_int64), ("B", ctypes.c_int64),
+                ("max_pages", ctypes.c_int64), ("table", ctypes.c_void_p),
+                ("table_host", ctypes.c_void_p), ("lens_dev", ctypes.c_void_p),
+                ("lens_host", ctypes.c_void_p)]
 
 
 _wsp = ctypes.POINTER(NneWorkspace)
@@ -153,6 +171,18 @@ SIGNATURES = {
         _vp, ctypes.c_int64, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64,
         ctypes.c_int64, _vp, _i32p, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64,
         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _wsp, _vp]),
+    "nne_qk_norm_rope": (ctypes.c_int, [
+        _vp, _i64p, _i64p, _vp, _i64p, _vp, _i64p, _i64p, _vp, _i64p, _vp, _vp, ctypes.c_int,
+        ctypes.c_float, _vp, _vp, ctypes.c_int64, ctypes.c_int64, _vp, _i32p, _vp, _i32p, _vp]),
+    "nne_paged_append": (ctypes.c_int, [
+        _vp, _vp, _i64p, _vp, _i64p, ctypes.c_int64, _vp, _i32p, _vp, _i32p, _vp, _vp,
+        ctypes.c_int64, ctypes.c_int64, _vp]),
+    "nne_paged_attention": (ctypes.c_int, [
+        _vp, _vp, _i64p, _vp, _i64p, ctypes.c_int64, ctypes.c_int64, _vp, _i32p, _vp, _i32p,
+        ctypes.c_int, ctypes.c_float, _wsp, _vp]),
+    "nne_paged_workspace_size": (ctypes.c_int, [_vp, ctypes.c_int64, ctypes.c_int64, _wszp]),
+    "nne_paged_commit": (ctypes.c_int, [
+        _vp, ctypes.c_int64, ctypes.c_int64, _vp, _i32p, _vp, _i32p, ctypes.c_int64, _wsp, _vp]),
 }
 
 
@@ -191,7 +221,11 @@ def _native_calls(l):
         attention=call(mod.attention, "nne_attention_forward_ws"),
         decode_attention=call(mod.decode_attention, "nne_decode_attention"),
         decode_step=call(mod.decode_step, "nne_decode_step"),
-        qkv_rope=call(mod.qkv_rope, "nne_qkv_rope_ws"))
+        qkv_rope=call(mod.qkv_rope, "nne_qkv_rope_ws"),
+        qk_norm_rope=call(mod.qk_norm_rope, "nne_qk_norm_rope"),
+        paged_append=call(mod.paged_append, "nne_paged_append"),
+        paged_attention=call(mod.paged_attention, "nne_paged_attention"),
+        paged_commit=call(mod.paged_commit, "nne_paged_commit"))
 
 
 def _native():
@@ -728,6 +762,455 @@ def qkv_rope(x, w_packed, bq, bk, bv, rope, pos_dev, pos_host, num_heads, num_kv
     return q_out, k_out, v_out
 
 
+def _on_device(device, *ts):
+    """The tensors are on ``device``, and it is the current one (whose streams
+    the calls run on)."""
+    import torch
+    for t in ts:
+        if t.device != device:
+            raise InvalidArgument("Invalid configuration or argument: expected tensors on %s, got %s"
+                                  % (device, t.device))
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise InvalidArgument("Invalid configuration or argument: %s is not the current device"
+                              % device)
+
+
+def _new_like(t, stream):
+    """An uninitialised contiguous tensor of t's shape, allocated for the stream
+    that writes it."""
+    import torch
+    if stream is None:
+        return t.new_empty(t.shape)
+    with torch.cuda.stream(stream):
+        return t.new_empty(t.shape)
+
+
+def _int_array(x, shape, what):
+    a = np.ascontiguousarray(x, dtype=np.int32)
+    if a.shape != shape:
+        raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s (%s)"
+                            % (list(shape), list(a.shape), what))
+    return a
+
+
+def _check_int_dev(t, shape, device, what):
+    import torch
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise InvalidArgument("Invalid configuration or argument: %s must be a contiguous int32 "
+                              "tensor of shape %s" % (what, list(shape)))
+    _on_device(device, t)
+
+
+class DraftTree:
+    """The tokens of one step for each of a batch's sequences, as a tree:
+    ``parents`` [B, T] holds, for token t, the token t' < t that it follows, or -1
+    where it follows the sequence's last row.  ``counts`` [B]: how many tokens of
+    each sequence exist (default: all T).  Positions and attention masks follow
+    from the parents; both arrays are copied to the device once, here."""
+
+    def __init__(self, parents, counts=None, device="cuda"):
+        parents = np.ascontiguousarray(parents, dtype=np.int32)
+        if parents.ndim != 2:
+            raise InvalidArgument("Invalid configuration or argument: parents must be [B, T], got %s"
+                                  % list(parents.shape))
+        self._set(parents.shape, counts, device)
+        b, t = parents.shape
+        exists = np.arange(t) < (np.full(b, t) if counts is None else self.counts_host)[:, None]
+        if (exists & ((parents < -1) | (parents >= np.arange(t)))).any():
+            raise InvalidArgument("Invalid configuration or argument: a token's parent comes before "
+                                  "it (-1: the sequence's last row)")
+        parents = np.where(exists, parents, -1).astype(np.int32)
+        depths = np.zeros((b, t), np.int32)
+        for i in range(1, t):
+            p = parents[:, i]
+            depths[:, i] = np.where(p < 0, 0, depths[np.arange(b), np.maximum(p, 0)] + 1)
+        self.parents_host, self.parents_dev = parents, self._dev(parents)
+        self.depths_host, self.depths_dev = depths, self._dev(depths)
+
+    @classmethod
+    def chain(cls, batch, tokens, counts=None, device="cuda"):
+        """Each token follows the one before: what a step without a DraftTree
+        is, with ``counts``."""
+        self = cls.__new__(cls)
+        self._set((int(batch), int(tokens)), counts, device)
+        self.parents_host = self.parents_dev = self.depths_host = self.depths_dev = None
+        return self
+
+    def _dev(self, a):
+        import torch
+        return torch.from_numpy(a).to(self.device)
+
+    def _set(self, shape, counts, device):
+        import torch
+        self.device = torch.empty(0, device=device).device
+        self.batch, self.tokens = shape
+        self.counts_host = self.counts_dev = None
+        if counts is not None:
+            self.counts_host = _int_array(counts, (self.batch,), "counts").copy()
+            if (self.counts_host < 0).any() or (self.counts_host > self.tokens).any():
+                raise InvalidArgument("Invalid configuration or argument: counts outside [0, %d]"
+                                      % self.tokens)
+            self.counts_dev = self._dev(self.counts_host)
+
+    @staticmethod
+    def _pair(dev, host):
+        return (None if dev is None else dev.data_ptr(), host)
+
+    def _check(self, batch, tokens, device):
+        if (self.batch, self.tokens) != (batch, tokens):
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                % ([self.batch, self.tokens], [batch, tokens]))
+        if self.device != device:
+            raise InvalidArgument("Invalid configuration or argument: expected tensors on %s, got %s"
+                                  % (device, self.device))
+
+    def _counts(self):
+        return self._pair(self.counts_dev, self.counts_host)
+
+    def _parents(self):
+        return self._pair(self.parents_dev, self.parents_host)
+
+    def _depths(self):
+        return self._pair(self.depths_dev, self.depths_host)
+
+
+_NO_PAIR = (None, None)
+_NO_ROPE = (None, None, 0, 0)
+
+
+def _rope_args(rope):
+    return _NO_ROPE if rope is None else (rope.cos.data_ptr(), rope.sin.data_ptr(),
+                                          rope.max_seq_len, rope.head_dim)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6, draft=None,
+                 q_out=None, k_out=None, stream=None):
+    """Per-head norm and rotation of queries and keys in one pass: each head x of
+    q [B, Hq, T, d] and k [B, Hkv, T, d] (any strides) becomes
+    RoPE(x / sqrt(mean(x^2) + eps) * weight), token t of sequence b at position
+    start[b] + t, or with a ``draft`` at start[b] + its depth in the tree
+    (``start``: int32 [B], device and host copies).  Weights are [d] or None (ones);
+    rope=None: no rotation; eps=None: no norm, the rotation alone (no weights);
+    k=None: q alone.  Returns (q_out, k_out): new contiguous tensors by default, or
+    the given ones (q and k themselves are fine)."""
+    _shape4(q, "Q")
+    tensors = [t for t in (q, k, q_weight, k_weight, q_out, k_out) if t is not None]
+    _require_f32_cuda(*tensors)
+    _on_device(q.device, *tensors)
+    b, _, t, d = q.shape
+    for w in (q_weight, k_weight):
+        if w is not None and (tuple(w.shape) != (d,) or not w.is_contiguous()):
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                % ([d], list(w.shape)))
+    if k is not None:
+        _shape4(k, "K")
+    for x, out in ((q, q_out), (k, k_out)):
+        if out is not None and (x is None or out.shape != x.shape):
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                % ([] if x is None else list(x.shape), list(out.shape)))
+    if q_out is None:
+        q_out = _new_like(q, stream)
+    if k is not None and k_out is None:
+        k_out = _new_like(k, stream)
+    start, depths = _NO_PAIR, _NO_PAIR
+    if rope is not None:
+        start_host = _int_array(start_host, (b,), "start_host")
+        _check_int_dev(start_dev, (b,), q.device, "start_dev")
+        _on_device(q.device, rope.cos, rope.sin)
+        start = (start_dev.data_ptr(), start_host)
+        if draft is not None:
+            draft._check(b, t, q.device)
+            depths = draft._depths()
+    ks = (None, (0, 0, 0, 0), (0, 0, 0, 0), None, (0, 0, 0, 0))
+    if k is not None:
+        ks = (k.data_ptr(), k.shape, k.stride(), k_out.data_ptr(), k_out.stride())
+    check(_native().qk_norm_rope(
+        q.data_ptr(), q.shape, q.stride(), q_out.data_ptr(), q_out.stride(), *ks,
+        None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), eps is not None,
+        float(eps or 0.0), *_rope_args(rope), *start, *depths, _stream(stream)))
+    return q_out, k_out
+
+
+class _StepWorkspace(Workspace):
+    """A workspace that captured graphs may refer to: buffers grow to powers of
+    two and replaced ones are kept, and nothing is allocated under capture (it
+    would belong to the graph, and its counters would not be cleared)."""
+
+    def __init__(self, device):
+        super().__init__(device)
+        self._kept = []
+
+    def reserve(self, size, stream=None):
+        import torch
+        have = (0 if self.records is None else self.records.numel(),
+                0 if self.counters is None else self.counters.numel())
+        if size.records_bytes <= have[0] and size.n_counters <= have[1]:
+            return self
+        if torch.cuda.is_current_stream_capturing():
+            raise InvalidArgument("Invalid configuration or argument: the workspace cannot grow "
+                                  "under capture; call reserve_workspace before")
+        grown = NneWorkspaceSize(*(1 << max(0, int(n) - 1).bit_length() if n else 0
+                                   for n in (size.records_bytes, size.n_counters)))
+        self._kept.append((self.records, self.counters))
+        with torch.cuda.stream(stream):       # (None: the current stream)
+            return super().reserve(grown, stream)
+
+
+class PagedKVCache:
+    """A KV cache of pages shared by many sequences (no counterpart in the
+    reference, whose caches are a tensor per layer, src/nn/kv_cache.rs:11-74).
+
+    ``k`` and ``v`` are the layers' pools [layers, pages, Hkv, page_size, d],
+    float32 or bfloat16 (d a multiple of 8 up to 256).  Row r of sequence b is row
+    r % page_size of page ``table_host[b, r // page_size]`` in every layer;
+    ``lens_host[b]`` rows count.  Tables and lengths are kept on the host
+    (validation, launch sizing) and on the device (read by kernels).
+
+    A step of one or more new tokens per sequence is, in each layer, ``append``
+    (their rows go behind the counted ones) and ``attend``; then once ``commit``,
+    which accepts new rows: all, the first few, or the path of a ``DraftTree``.
+    Until then a further append writes the same rows again."""
+
+    def __init__(self, num_layers, num_pages, num_kv_heads, page_size, head_dim, batch,
+                 max_pages_per_seq, dtype=None, device="cuda"):
+        import torch
+        self.num_kv_heads, self.head_dim = int(num_kv_heads), int(head_dim)
+        self.num_pages, self.page_size = int(num_pages), int(page_size)
+        self.batch, self.max_pages = int(batch), int(max_pages_per_seq)
+        self.dtype = torch.float32 if dtype is None else dtype
+        if self.dtype not in (torch.float32, torch.bfloat16):
+            raise InvalidArgument("Invalid configuration or argument: a paged cache holds float32 or "
+                                  "bfloat16, not %s" % self.dtype)
+        if min(self.num_kv_heads, self.head_dim, self.num_pages, self.page_size,
+               self.max_pages) <= 0 or self.batch < 0 or num_layers < 0:
+            raise InvalidArgument("Invalid configuration or argument: bad paged cache geometry")
+        shape = (int(num_layers), self.num_pages, self.num_kv_heads, self.page_size, self.head_dim)
+        self._shape = shape
+        self._k = torch.zeros(shape, dtype=self.dtype, device=device)
+        self._v = torch.zeros(shape, dtype=self.dtype, device=device)
+        self._device = self._k.device
+        self.table_host = np.full((self.batch, self.max_pages), -1, np.int32)
+        self.table_dev = torch.full((self.batch, self.max_pages), -1, dtype=torch.int32,
+                                    device=device)
+        self.lens_host = np.zeros(self.batch, np.int32)
+        self.lens_dev = torch.zeros(self.batch, dtype=torch.int32, device=device)
+        self._ws = _StepWorkspace(self._device)
+        self._sizes = {}
+        self._bind()
+
+    @property
+    def k(self):
+        return self._k
+
+    @k.setter
+    def k(self, pool):
+        self._k = self._check_pool(pool)
+        self._bind()
+
+    @property
+    def v(self):
+        return self._v
+
+    @v.setter
+    def v(self, pool):
+        self._v = self._check_pool(pool)
+        self._bind()
+
+    def _check_pool(self, pool):
+        if tuple(pool.shape) != self._shape:
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                % (list(self._shape), list(pool.shape)))
+        if pool.dtype != self.dtype or pool.device != self._device or not pool.is_contiguous():
+            raise InvalidArgument("Invalid configuration or argument: a pool is a contiguous %s tensor "
+                                  "on %s" % (self.dtype, self._device))
+        return pool
+
+    def _bind(self):
+        """The layers' nne_paged_cache_t.  Attention reads pages of rows that were
+        checked when the table, the lengths or the rows came; appending checks."""
+        import torch
+        size = 2 if self.dtype == torch.bfloat16 else 4
+        self._layer_stride = self.num_pages * self.num_kv_heads * self.page_size * self.head_dim
+        step = self._layer_stride * size
+        k, v = self._k.data_ptr(), self._v.data_ptr()
+
+        def struct(i, table_host):
+            return NnePagedCache(k + i * step, v + i * step, int(size == 2), self.num_pages,
+                                 self.num_kv_heads, self.page_size, self.head_dim, self.batch,
+                                 self.max_pages, self.table_dev.data_ptr(), table_host,
+                                 self.lens_dev.data_ptr(), self.lens_host.ctypes.data)
+
+        host = self.table_host.ctypes.data
+        self._structs = [(struct(i, host), struct(i, None)) for i in range(self._shape[0])]
+        self._addr = [tuple(ctypes.addressof(s) for s in pair) for pair in self._structs]
+
+    def num_layers(self):
+        return self._shape[0]
+
+    def capacity(self):
+        """Rows a sequence's pages can hold."""
+        return self.max_pages * self.page_size
+
+    def _check_layer(self, layer_idx):
+        if not 0 <= layer_idx < self._shape[0]:
+            raise InvalidArgument(
+                "Invalid configuration or argument: PagedKVCache layer index %d out of range "
+                "(total layers: %d)" % (layer_idx, self._shape[0]))
+
+    def _check_pages(self, table, lens):
+        if (table < -1).any() or (table >= self.num_pages).any():
+            raise InvalidArgument("Invalid configuration or argument: page outside [0, %d)"
+                                  % self.num_pages)
+        used = np.arange(self.max_pages) < -(-lens.astype(np.int64) // self.page_size)[:, None]
+        if (used & (table < 0)).any():
+            raise InvalidArgument("Invalid configuration or argument: a counted row has no page")
+
+    def set_table(self, table):
+        """Sets every sequence's pages: [B, n] page numbers, n at most
+        max_pages_per_seq, -1 for none.  Sequences may share pages of rows that
+        no longer change (append refuses a page for two sequences' new rows)."""
+        import torch
+        table = np.asarray(table)
+        if table.ndim != 2 or table.shape[0] != self.batch or table.shape[1] > self.max_pages:
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                % ([self.batch, self.max_pages], list(table.shape)))
+        full = np.full_like(self.table_host, -1)
+        full[:, :table.shape[1]] = table
+        self._check_pages(full, self.lens_host)
+        self.table_host[...] = full
+        self.table_dev.copy_(torch.from_numpy(full))
+
+    def set_lengths(self, lens):
+        """Declares that rows [0, lens[b]) of every sequence are filled."""
+        import torch
+        lens = np.asarray(lens, dtype=np.int32)
+        if lens.shape != (self.batch,) or (lens < 0).any() or (lens > self.capacity()).any():
+            raise InvalidArgument("Invalid configuration or argument: bad lengths")
+        self._check_pages(self.table_host, lens)
+        self.lens_host[:] = lens
+        self.lens_dev.copy_(torch.from_numpy(lens.copy()))
+
+    def allocate(self, rows):
+        """Gives every sequence pages for rows[b] rows (an int: the same for
+        all), out of those that no sequence has.  Pages it has stay.
+        CapacityError (nothing changed) where the pool or a table row is full."""
+        rows = np.broadcast_to(np.asarray(rows, np.int64), (self.batch,))
+        if (rows > self.capacity()).any():
+            raise CapacityError("GPU compute error: %d rows exceed %d pages of %d rows"
+                                % (rows.max(), self.max_pages, self.page_size))
+        table = self.table_host.copy()
+        free = np.setdiff1d(np.arange(self.num_pages, dtype=np.int32), table)
+        wanted = (np.arange(self.max_pages) < -(-rows // self.page_size)[:, None]) & (table < 0)
+        if int(wanted.sum()) > len(free):
+            raise CapacityError("GPU compute error: %d pages wanted, %d of %d are free"
+                                % (wanted.sum(), len(free), self.num_pages))
+        table[wanted] = free[:int(wanted.sum())]
+        self.set_table(table)
+
+    def release(self, seq):
+        """Ends a sequence: no rows, no pages."""
+        if not 0 <= seq < self.batch:
+            raise InvalidArgument("Invalid configuration or argument: sequence %d of %d"
+                                  % (seq, self.batch))
+        lens, table = self.lens_host.copy(), self.table_host.copy()
+        lens[seq], table[seq] = 0, -1
+        self.set_lengths(lens)
+        self.set_table(table)
+
+    def _size(self, num_heads, tokens):
+        key = (num_heads, tokens)
+        if key not in self._sizes:
+            size = NneWorkspaceSize()
+            s = NnePagedCache.from_buffer_copy(self._structs[0][1]) if self._structs else None
+            check(lib().nne_paged_workspace_size(None if s is None else ctypes.addressof(s),
+                                                 num_heads, tokens, ctypes.byref(size)))
+            self._sizes[key] = size
+        return self._sizes[key]
+
+    def reserve_workspace(self, num_heads, tokens, stream=None):
+        """Grows the cache's workspace to steps of ``tokens`` tokens and
+        ``num_heads`` query heads, as a step under capture needs it to be."""
+        self._ws.reserve(self._size(int(num_heads), int(tokens)), stream)
+
+    def append(self, layer_idx, k_new, v_new, rope=None, draft=None, stream=None):
+        """Writes the rows of new tokens, k_new / v_new [B, Hkv, T, d] (any
+        strides), behind the counted rows, the keys rotated at their tokens'
+        positions (``rope``: a RotaryEmbedding; None: as they are)."""
+        self._check_layer(layer_idx)
+        _require_f32_cuda(k_new, v_new)
+        _on_device(self._device, k_new, v_new)
+        _shape4(k_new, "K")
+        b, h, t, d = k_new.shape
+        if (b, h, d) != (self.batch, self.num_kv_heads, self.head_dim) or v_new.shape != k_new.shape:
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s" % (
+                [self.batch, self.num_kv_heads, t, self.head_dim],
+                list(v_new.shape if v_new.shape != k_new.shape else k_new.shape)))
+        counts = depths = _NO_PAIR
+        if draft is not None:
+            draft._check(b, t, self._device)
+            counts, depths = draft._counts(), draft._depths()
+        if rope is not None:
+            _on_device(self._device, rope.cos, rope.sin)
+        check(_native().paged_append(
+            self._addr[layer_idx][0], k_new.data_ptr(), k_new.stride(), v_new.data_ptr(),
+            v_new.stride(), t, *counts, *depths, *_rope_args(rope), _stream(stream)))
+
+    def attend(self, layer_idx, q, draft=None, out=None, scale=None, stream=None):
+        """Attention of the appended tokens' queries q [B, Hq, T, d] over the
+        counted rows and those new ones that lead to them.  Rows of ``out`` for
+        tokens past a draft's counts are left as they were (undefined in a new
+        ``out``)."""
+        self._check_layer(layer_idx)
+        _shape4(q, "Q")
+        _require_f32_cuda(q)
+        _on_device(self._device, q)
+        b, hq, t, d = q.shape
+        if (b, d) != (self.batch, self.head_dim) or hq == 0 or hq % self.num_kv_heads != 0:
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s" % (
+                [self.batch, self.num_kv_heads, t, self.head_dim], list(q.shape)))
+        if out is None:
+            out = _new_like(q, stream)
+        else:
+            _require_f32_cuda(out)
+            _on_device(self._device, out)
+            if out.shape != q.shape:
+                raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                    % (list(q.shape), list(out.shape)))
+        counts = parents = _NO_PAIR
+        if draft is not None:
+            draft._check(b, t, self._device)
+            counts, parents = draft._counts(), draft._parents()
+        check(_native().paged_attention(
+            self._addr[layer_idx][1], q.data_ptr(), q.stride(), out.data_ptr(), out.stride(), hq, t,
+            *counts, *parents, scale is not None, float(scale or 0.0),
+            _ws_arg(self._ws, self._size(hq, t), stream), _stream(stream)))
+        return out
+
+    def commit(self, counts, counts_host=None, paths=None, paths_host=None, stream=None):
+        """Accepts new rows in every layer.  counts: an int (every sequence's
+        first ``counts`` tokens), or int32 [B] on the device with its host copy.
+        paths (int32 [B, J], device and host copies): the accepted tokens of a
+        tree, ascending; their rows move behind the counted ones."""
+        if isinstance(counts, (int, np.integer)):
+            host = np.full(self.batch, counts, np.int32)
+            dev = None
+        else:
+            _check_int_dev(counts, (self.batch,), self._device, "counts")
+            host = _int_array(counts_host, (self.batch,), "counts_host")
+            dev = counts.data_ptr()
+        j, path = int(host.max()) if self.batch else 0, _NO_PAIR
+        if paths is not None:
+            j = int(paths.shape[-1])
+            _check_int_dev(paths, (self.batch, j), self._device, "paths")
+            path = (paths.data_ptr(), _int_array(paths_host, (self.batch, j), "paths_host"))
+        if not self._addr:
+            raise InvalidArgument("Invalid configuration or argument: a cache of no layers")
+        check(_native().paged_commit(
+            self._addr[0][0], self._shape[0], self._layer_stride, dev, host, *path, max(j, 0),
+            _ws_arg(self._ws, NneWorkspaceSize(0, self.batch), stream), _stream(stream)))
+
+
 class GroupedQueryAttention:
     """GroupedQueryAttention (src/models/llama.rs:160-300), forward only.
 
@@ -761,6 +1244,39 @@ class GroupedQueryAttention:
         self.w_packed = None
         if self.head_dim % 64 == 0 and d_model % 64 == 0:
             self.w_packed = qkv_pack(self.wq, self.wk, self.wv, num_heads, num_kv_heads)
+        self.q_norm = self.k_norm = self.norm_eps = None
+
+    def set_qk_norm(self, q_weight, k_weight, eps=1e-6):
+        """Norms the heads of q and k before the rotation (weights [d]); taken by
+        forward_gqa_paged alone."""
+        self.q_norm, self.k_norm, self.norm_eps = q_weight, k_weight, float(eps)
+
+    def forward_gqa_paged(self, x, cache, layer_idx=0, draft=None, stream=None):
+        """A step over a PagedKVCache: x [B, T, C] holds T new tokens of every
+        sequence (a chain, or a DraftTree's); their rows are appended and not yet
+        counted -- the caller commits once, after the last layer."""
+        import torch
+        if x.dim() != 3:
+            raise EngineError("Incompatible shapes for operation GroupedQueryAttention forward "
+                              "(expected 3D input [B, T, C]): %s" % [list(x.shape)])
+        b, t, c = x.shape
+        hq, hkv, d = self.num_heads, self.num_kv_heads, self.head_dim
+        cache._check_layer(layer_idx)
+        with torch.cuda.stream(stream):        # (None: the current stream)
+            q = torch.nn.functional.linear(x, self.wq).view(b, t, hq, d).transpose(1, 2)
+            k = torch.nn.functional.linear(x, self.wk).view(b, t, hkv, d).transpose(1, 2)
+            v = torch.nn.functional.linear(x, self.wv).view(b, t, hkv, d).transpose(1, 2)
+            out = torch.zeros((b, t, hq, d), dtype=torch.float32, device=x.device)
+            start = (cache.lens_dev, cache.lens_host)
+            if self.norm_eps is not None:
+                q, k = qk_norm_rope(q, k, self.q_norm, self.k_norm, self.rope, *start,
+                                    eps=self.norm_eps, draft=draft)
+                cache.append(layer_idx, k, v, draft=draft)
+            else:
+                q, _ = qk_norm_rope(q, None, None, None, self.rope, *start, eps=None, draft=draft)
+                cache.append(layer_idx, k, v, rope=self.rope, draft=draft)
+            cache.attend(layer_idx, q, draft=draft, out=out.transpose(1, 2))
+            return torch.nn.functional.linear(out.view(b, t, hq * d), self.wo)
 
     def forward_gqa_cached(self, x, start_pos, cache=None, layer_idx=0, stream=None):
         """x [B, T, C].  With a cache, start_pos must be each sequence's cached

@@ -22,7 +22,7 @@ LIB = os.path.join(LIB_DIR, "libnne_attn.so")
 HOST_LIB = os.path.join(LIB_DIR, "libnne_host.so")
 CALL_LIB = os.path.join(LIB_DIR, "nne_pycall.so")
 
-SOURCES = ["prefill.hip", "small.hip", "splitk.hip", "splitk_plan.cpp", "qkv.hip", "deep.hip", "deep_plan.cpp", "abi.cpp", "noalloc.hip"]
+SOURCES = ["prefill.hip", "small.hip", "splitk.hip", "splitk_plan.cpp", "qkv.hip", "deep.hip", "deep_plan.cpp", "abi.cpp", "noalloc.hip", "paged.hip", "paged_attn.hip", "paged_plan.cpp", "paged_abi.cpp"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -141,6 +141,19 @@ hipError_t stream_resources(int64_t n, uint64_t ws_bytes, hipStream_t s, uint32_
     return hipSuccess;
 }
 
+// Whether the stream's resources hold n counters and ws_bytes already.
+bool stream_holds(int64_t n, uint64_t ws_bytes, hipStream_t s) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    const std::thread::id th =
+        s == hipStreamPerThread ? std::this_thread::get_id() : std::thread::id();
+    std::lock_guard<std::mutex> lock(g_res_mu);
+    for (const auto& x : g_res)
+        if (x.dev == dev && x.stream == s && x.thread == th)
+            return x.n_counters >= n && x.ws_bytes >= ws_bytes;
+    return false;
+}
+
 // Records and counters of one call: the caller's workspace, checked against
 // what the call needs, or (ws == NULL) the stream's library-side ones.
 int call_workspace(const nne_workspace_t* ws, uint64_t need_bytes, int64_t need_counters,
@@ -489,6 +502,31 @@ namespace nne {
 int fail_message(int code, const char* msg) { return fail(code, "%s", msg); }
 
 int fail_hip(hipError_t e, const char* what) { return hip_fail(e, what); }
+
+int fail_format(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+
+void row_major_strides(const int64_t* shape, int64_t* strides) { contiguous_strides(shape, strides); }
+
+int cus_of_device() { return device_cus(); }
+
+int take_workspace(const nne_workspace_t* ws, uint64_t need_bytes, int64_t need_counters,
+                   hipStream_t s, void** records, uint32_t** counters, const char* what) {
+    if (!ws) {
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        if (s && hipStreamIsCapturing(s, &st) == hipSuccess && st == hipStreamCaptureStatusActive &&
+            !stream_holds(need_counters, need_bytes, s))
+            return fail(NNE_EINVAL, "Invalid configuration or argument: %s on a stream under capture needs "
+                                    "a workspace, or an earlier call of this size on the stream", what);
+    }
+    return call_workspace(ws, need_bytes, need_counters, s, records, counters, what);
+}
 
 }  // namespace nne
 

@@ -21,4 +21,20 @@ int run_decode(const float* q, const int64_t* q_strides, const float* k_cache, c
                const int64_t* o_strides, int64_t B, int64_t Hq, int64_t Hkv, int64_t capacity,
                int64_t d, int has_scale, float scale, const nne_workspace_t* ws, hipStream_t s);
 
+// nne_last_error() message in printf form; returns `code`.
+int fail_format(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// Row-major strides of a [n0, n1, n2, n3] tensor.
+void row_major_strides(const int64_t* shape, int64_t* strides);
+
+// CUs of the current device.
+int cus_of_device();
+
+// Records and counters of one call: the caller's workspace, checked against the
+// call's needs, or (ws == NULL) the stream's library-side ones.  A stream under
+// capture is refused one that would have to be allocated: the allocation would
+// become a node of the graph.
+int take_workspace(const nne_workspace_t* ws, uint64_t need_bytes, int64_t need_counters,
+                   hipStream_t s, void** records, uint32_t** counters, const char* what);
+
 }  // namespace nne

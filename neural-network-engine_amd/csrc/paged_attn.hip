@@ -1,0 +1,578 @@
+// Attention over a paged KV cache: a step's new tokens -- one, a chain, or a
+// tree -- against their sequence's rows and the new ones on their path.
+//
+//   o[r] = sum_c 2^(s[r,c] - m[r]) v[c] / sum_c 2^(s[r,c] - m[r]),
+//   s[r,c] = (scale log2(e) q[r]) . k[c] where r sees c, else -inf,
+//
+// in one pass over the keys with the running maximum m and sum per row.
+//
+// A KV head's G * T query rows (row r: token r / G of query head r % G) are the
+// columns of MFMA tiles, its keys the rows:  S^T = K Q^T, O^T += V^T P^T.  Both
+// products take K and V from registers as they come from memory, with no LDS:
+//   * K: lane l (column l % 16, group g = l / 16) holds dims of key l % 16;
+//     which dims sit in which step does not matter as long as Q agrees;
+//   * S^T arrives as 4 keys (4 g + i) of row l % 16 per lane, which is how the
+//     second product takes P^T, if its step pairs those keys: lane group g loads
+//     V rows 4 g + i, and the lane's consecutive dims become the tiles' rows.
+// f32 pools run on the f32 MFMAs (16x16x4, exact products, 16 keys a block).
+// bf16 pools run on the bf16 MFMAs (16x16x32, 32 keys a block): K and V are
+// exact there, Q and P are the exact sums of three bf16 parts, so products are
+// exact and sums f32, at three MFMAs a product.  P's parts lose bits only of
+// weights below 2^-110 of the row's largest.
+//
+// A workgroup is 4 waves that take blocks of its part of the keys in turn and
+// meet only at the end.  Parts of a sequence (paged_plan.cpp) leave records that
+// the last workgroup to arrive merges in the order of the parts, so results do
+// not depend on who that is.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged_device.hpp"
+#include "paged_launch.hpp"
+
+namespace nne {
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr int kStage = 2048;     // keys whose pool rows are in LDS at a time
+
+__device__ __forceinline__ float row_groups_max(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    return pair_max(x);
+}
+__device__ __forceinline__ float row_groups_sum(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    return pair_sum(x);
+}
+
+__device__ __forceinline__ floatx4 mfma_part(uintx4 a, uintx4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool NT, typename V>
+__device__ __forceinline__ V load_vec(const void* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(static_cast<const V*>(p));
+    else return *static_cast<const V*>(p);
+}
+
+// What differs between the pools' types.  KB: keys of a block, JN: keys of a
+// block per lane, VE: consecutive dims of a V load.
+template <bool BF16, int D>
+struct Shape {
+    static constexpr int KB = BF16 ? 32 : 16;
+    static constexpr int JN = KB / 4;
+    static constexpr int VE = BF16 ? (D >= 128 ? 8 : 4) : 4;
+    static constexpr int NV = D / (16 * VE);          // V loads per key
+    static constexpr int KT = KB / 16;                // 16-key tiles
+    static constexpr int KS = BF16 ? D / 32 : D / 16; // K loads per tile
+    static constexpr int NO = D / 16;                 // 16-dim tiles of O
+    static constexpr int ES = BF16 ? 2 : 4;           // bytes of an element
+};
+
+// Key of a block that slot j of lane group g stands for.
+template <bool BF16>
+__device__ __forceinline__ int slot_key(int g, int j) {
+    return BF16 ? 16 * (j >> 2) + 4 * g + (j & 3) : 4 * g + j;
+}
+
+__device__ __forceinline__ bool not_finite(float x) {
+    return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+}
+
+// BF16: the pools' type.  D: dims, padded.  NRT: 16-row tiles of query rows.
+// FULL: d == D.  NT: no other workgroup reads these keys.
+template <bool BF16, int D, int NRT, bool FULL, bool NT>
+__global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_attention_kernel(const PagedAttnParams p) {
+    using S = Shape<BF16, D>;
+    constexpr int KB = S::KB, JN = S::JN, VE = S::VE, NV = S::NV, KT = S::KT, KS = S::KS, NO = S::NO;
+    constexpr int OS = D + 4;                        // row stride of the merge buffer
+    constexpr int ROWS = 16 * NRT;
+
+    __shared__ __attribute__((aligned(16))) float ob[4 * 16 * OS];
+    __shared__ __attribute__((aligned(16))) int rows_s[kStage];
+    __shared__ float ml_s[4][16][2];
+    __shared__ uint32_t anc_s[kPagedTreeNodes][kPagedTreeNodes / 32];
+    __shared__ int nxt_s[kPagedTreeNodes];
+    __shared__ int last_s, odd_s;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const PagedPool& pool = p.pool;
+
+    // Workgroup -> (part and KV head, row block).  With several row blocks, the
+    // ones that read the same keys follow each other on one XCD (workgroups go to
+    // the 8 XCDs in turn), whose L2 then serves them.
+    int unit = blockIdx.x, rb = 0;
+    if (p.n_rb > 1) {
+        const int x = unit & 7, y = unit >> 3;
+        rb = y % p.n_rb;
+        unit = (y / p.n_rb) * 8 + x;
+    }
+    if (unit >= p.prefix[p.B] * pool.Hkv) return;
+    const int part_all = unit / pool.Hkv, h = unit % pool.Hkv;
+    int bl;
+    {
+        const int lo = lane < p.B ? p.prefix[lane + 1] : INT32_MAX;
+        const int hi = lane + 64 < p.B ? p.prefix[lane + 65] : INT32_MAX;
+        bl = __popcll(__builtin_amdgcn_ballot_w64(lo <= part_all)) +
+             __popcll(__builtin_amdgcn_ballot_w64(hi <= part_all));
+    }
+    const int part = part_all - p.prefix[bl], n_parts = p.prefix[bl + 1] - p.prefix[bl];
+    const int b = p.b0 + bl;
+
+    const int row0 = rb * ROWS;
+    const int n_rows = min(ROWS, p.R - row0);
+    const int len = paged_len(pool, b);
+    const int count = paged_count(p.counts, b, p.T);
+    if (row0 / p.G >= count) return;                 // no token of this block exists
+    // Keys that some row sees, cut into equal parts of whole 32-key steps.
+    const int seen = p.parents ? count : min(count, (row0 + n_rows - 1) / p.G + 1);
+    const int n_keys = len + seen;
+    const int part_len = ((n_keys + n_parts - 1) / n_parts + 31) & ~31;
+    const int k0 = part * part_len, k1 = min(n_keys, k0 + part_len);
+    if (k0 >= k1) return;                            // part 0 always has keys
+    const int live = (n_keys + part_len - 1) / part_len;
+
+    // Q^T: the second operand of S^T, scaled; row col of tile rt.
+    uintx4 qb[BF16 ? NRT : 1][BF16 ? KS : 1][3];
+    vf4 qf[BF16 ? 1 : NRT][BF16 ? 1 : KS];
+    int tok[NRT];
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+        const int r = min(row0 + 16 * rt + col, p.R - 1);
+        const bool rok = 16 * rt + col < n_rows;
+        tok[rt] = r / p.G;
+        const float* qp = p.q.p + b * p.q.sb + (h * p.G + r % p.G) * p.q.sh + tok[rt] * p.q.st;
+        auto dims4 = [&](int c) __attribute__((always_inline)) {
+            vf4 x = vf4{0.f, 0.f, 0.f, 0.f};
+            if (rok && (FULL || c < pool.d))
+                x = p.vec_q ? *reinterpret_cast<const vf4*>(qp + c)
+                            : vf4{qp[c * p.q.sd], qp[(c + 1) * p.q.sd], qp[(c + 2) * p.q.sd], qp[(c + 3) * p.q.sd]};
+            return x * p.qscale;
+        };
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (BF16) {
+                const vf4 x = dims4(32 * s + 8 * g), y = dims4(32 * s + 8 * g + 4);
+                uint32_t w[3][4];
+                split3(x[0], x[1], w[0][0], w[1][0], w[2][0]);
+                split3(x[2], x[3], w[0][1], w[1][1], w[2][1]);
+                split3(y[0], y[1], w[0][2], w[1][2], w[2][2]);
+                split3(y[2], y[3], w[0][3], w[1][3], w[2][3]);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) qb[rt][s][i] = uintx4{w[i][0], w[i][1], w[i][2], w[i][3]};
+            } else {
+                qf[rt][s] = dims4(16 * s + 4 * g);
+            }
+        }
+    }
+
+    if (tid == 0) odd_s = 0;             // (the stage's barriers follow)
+
+    // Which drafted tokens precede a token: bit u of anc_s[t].  Pointer
+    // doubling: after k rounds a row holds its 2^k nearest.
+    if (p.parents && k1 > len) {
+        constexpr int W = kPagedTreeNodes / 32;
+        const int words = (p.T + 31) / 32;
+        uint32_t own[W];
+        int next = -1;
+        if (tid < p.T) {
+            next = p.parents[(int64_t)b * p.T + tid];
+            if (next >= tid) next = -1;
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) own[w] = w == tid >> 5 ? 1u << (tid & 31) : 0u;
+        for (int span = 1;; span *= 2) {
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                if (w < words) anc_s[tid][w] = own[w];
+            nxt_s[tid] = next;
+            __syncthreads();
+            if (span >= p.T) break;
+            const int at = next;
+            if (at >= 0) {
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+                    if (w < words) own[w] |= anc_s[at][w];
+                next = nxt_s[at];
+            }
+            __syncthreads();
+        }
+    }
+    // Whether token t sees drafted token u (u < 0: a counted row).  Without
+    // branches: lanes differ.
+    auto sees = [&](int t, int u) __attribute__((always_inline)) -> bool {
+        if (!p.parents) return u <= t;
+        const int at = min(max(u, 0), kPagedTreeNodes - 1);
+        return (u < 0) | (((anc_s[t][at >> 5] >> (at & 31)) & 1u) != 0);
+    };
+
+    floatx4 o[NRT][NO];
+    float m_run[NRT], l_run[NRT];
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+        m_run[rt] = kNegInf;
+        l_run[rt] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NO; ++c) o[rt][c] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // Dims past d: any of the row's own (their Q is zero, their O is not kept).
+    const auto clamp_dim = [&](int c) __attribute__((always_inline)) { return FULL || c < pool.d ? c : 0; };
+    const char* const kbase = static_cast<const char*>(pool.k);
+    const char* const vbase = static_cast<const char*>(pool.v);
+    const int64_t row_bytes = (int64_t)pool.d * S::ES;
+    typedef typename std::conditional<BF16 && VE == 4, uintx2, uintx4>::type VReg;
+
+    const int32_t* const table = pool.table + (int64_t)b * pool.max_pages;
+    for (int kc = k0; kc < k1; kc += kStage) {
+        const int n_stage = min(kStage, k1 - kc);
+        const int n_blocks = (n_stage + KB - 1) / KB;
+        if (kc > k0) __syncthreads();
+        bool bad = false;
+        for (int i = tid; i < n_blocks * KB; i += 256) {
+            int row = -1;
+            if (i < n_stage) {
+                row = paged_row(pool, table, h, kc + i);
+                bad |= row < 0;
+            }
+            rows_s[i] = row;
+        }
+        const bool holes = __syncthreads_or(bad) != 0;
+
+        uintx4 kreg[KT][KS];
+        VReg vreg[JN][NV];
+        auto load_k = [&](int blk) __attribute__((always_inline)) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const char* row = kbase + max(rows_s[blk * KB + 16 * kt + col], 0) * row_bytes;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    kreg[kt][s] = load_vec<NT, uintx4>(row + S::ES * clamp_dim(BF16 ? 32 * s + 8 * g : 16 * s + 4 * g));
+            }
+        };
+        auto load_v = [&](int blk) __attribute__((always_inline)) {
+#pragma unroll
+            for (int q = 0; q < JN / 4; ++q) {
+                const intx4 r4 = *reinterpret_cast<const intx4*>(rows_s + blk * KB + 16 * q + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const char* row = vbase + max(r4[i], 0) * row_bytes;
+#pragma unroll
+                    for (int c = 0; c < NV; ++c)
+                        vreg[4 * q + i][c] = load_vec<NT, VReg>(row + S::ES * clamp_dim(16 * VE * c + VE * col));
+                }
+            }
+        };
+
+        int blk = wave;
+        if (blk < n_blocks) {
+            load_k(blk);
+            load_v(blk);
+        }
+        for (; blk < n_blocks; blk += 4) {
+            const int kb = kc + blk * KB;
+            // ---- S^T = K Q^T
+            floatx4 s[NRT][KT];
+#pragma unroll
+            for (int rt = 0; rt < NRT; ++rt)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) s[rt][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < KS; ++st)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int rt = 0; rt < NRT; ++rt) {
+                        if constexpr (BF16) {
+#pragma unroll
+                            for (int i = 2; i >= 0; --i) s[rt][kt] = mfma_part(kreg[kt][st], qb[rt][st][i], s[rt][kt]);
+                        } else {
+                            const vf4 kv = __builtin_bit_cast(vf4, kreg[kt][st]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qf[rt][st][i], s[rt][kt], 0, 0, 0);
+                        }
+                    }
+            const bool more = blk + 4 < n_blocks;
+            if (more) load_k(blk + 4);
+
+            // ---- masks: only the last blocks have any
+            const bool drafted = p.T > 1 && kb + KB > len;
+            if (holes || kb + KB > k1 || drafted) {
+#pragma unroll
+                for (int j = 0; j < JN; ++j) {
+                    const int in = slot_key<BF16>(g, j);
+                    const bool there = rows_s[blk * KB + in] >= 0;
+#pragma unroll
+                    for (int rt = 0; rt < NRT; ++rt) {
+                        const bool ok = there & (!drafted | sees(tok[rt], kb + in - len));
+                        const float x = s[rt][j >> 2][j & 3];
+                        s[rt][j >> 2][j & 3] = ok ? x : kNegInf;
+                    }
+#pragma unroll
+                    for (int c = 0; c < NV; ++c)
+#pragma unroll
+                        for (int w = 0; w < (int)(sizeof(VReg) / 4); ++w) vreg[j][c][w] = there ? vreg[j][c][w] : 0u;
+                }
+            }
+
+            // ---- softmax: 2^(s - m), row col's other keys are in lanes l ^ 16, l ^ 32
+            bool grow = false;
+            float m_blk[NRT];
+#pragma unroll
+            for (int rt = 0; rt < NRT; ++rt) {
+                float m = s[rt][0][0];
+#pragma unroll
+                for (int j = 1; j < JN; ++j) m = fmaxf(m, s[rt][j >> 2][j & 3]);
+                m_blk[rt] = row_groups_max(m);
+                grow |= m_blk[rt] > m_run[rt];
+            }
+            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+                for (int rt = 0; rt < NRT; ++rt) {
+                    const float m_new = fmaxf(m_run[rt], m_blk[rt]);
+                    const float alpha = fast_exp2(m_run[rt] - (m_new == kNegInf ? 0.f : m_new));
+                    m_run[rt] = m_new;
+                    l_run[rt] *= alpha;
+#pragma unroll
+                    for (int c = 0; c < NO; ++c) o[rt][c] *= alpha;
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < NRT; ++rt) {
+                const float m_use = m_run[rt] == kNegInf ? 0.f : m_run[rt];
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < JN; ++j) {
+                    const float w = fast_exp2(s[rt][j >> 2][j & 3] - m_use);
+                    s[rt][j >> 2][j & 3] = w;
+                    sum += w;
+                }
+                l_run[rt] += sum;
+            }
+
+            // ---- where rows see different keys: a V that is not finite would
+            // reach the rows that do not see it as 0 * inf.  Such values are taken
+            // out here and added to the rows that see them at the end.
+            if (drafted) {
+                bool odd = false;
+#pragma unroll
+                for (int j = 0; j < JN; ++j)
+#pragma unroll
+                    for (int c = 0; c < NV; ++c)
+#pragma unroll
+                        for (int w = 0; w < (int)(sizeof(VReg) / 4); ++w) {
+                            const uint32_t x = vreg[j][c][w];
+                            const bool lo = BF16 && (x & 0x7f80u) == 0x7f80u, hi = (x & 0x7f800000u) == 0x7f800000u;
+                            odd |= lo | hi;
+                            vreg[j][c][w] = x & (lo ? 0xffff0000u : ~0u) & (hi ? (BF16 ? 0x0000ffffu : 0u) : ~0u);
+                        }
+                if (odd) odd_s = 1;
+            }
+
+            // ---- O^T += V^T P^T
+            if constexpr (BF16) {
+                uintx4 vt[NO];               // dim c % VE of each load, two keys a register
+#pragma unroll
+                for (int c = 0; c < NO; ++c)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        vt[c][k] = __builtin_amdgcn_perm(vreg[2 * k + 1][c / VE][(c % VE) / 2], vreg[2 * k][c / VE][(c % VE) / 2],
+                                                         c % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int rt = 0; rt < NRT; ++rt) {
+                    uint32_t w[3][4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        split3(s[rt][k >> 1][2 * (k & 1)], s[rt][k >> 1][2 * (k & 1) + 1], w[0][k], w[1][k], w[2][k]);
+#pragma unroll
+                    for (int i = 2; i >= 0; --i) {
+                        const uintx4 pb = uintx4{w[i][0], w[i][1], w[i][2], w[i][3]};
+#pragma unroll
+                        for (int c = 0; c < NO; ++c) o[rt][c] = mfma_part(vt[c], pb, o[rt][c]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < JN; ++j)
+#pragma unroll
+                    for (int c = 0; c < NO; ++c) {
+                        const float v = __builtin_bit_cast(vf4, vreg[j][c / 4])[c % 4];
+#pragma unroll
+                        for (int rt = 0; rt < NRT; ++rt)
+                            o[rt][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[rt][0][j], o[rt][c], 0, 0, 0);
+                    }
+            }
+            if (more) load_v(blk + 4);
+        }
+    }
+
+    // ---- the 4 waves' (m, l, O), one tile of rows at a time
+    const int64_t rec_floats = paged_record_floats(p.rec_rows, D);
+    const int o_at = (2 * p.rec_rows + 3) & ~3;          // O of a record
+    const int heads_blocks = pool.Hkv * p.n_rb;
+    const int64_t rec0 = ((int64_t)p.prefix[bl] * pool.Hkv + h) * p.n_rb + rb;   // part 0's record
+    float* const rec = p.ws + (rec0 + (int64_t)part * heads_blocks) * rec_floats;
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) {
+        if (16 * rt >= n_rows) break;
+        const float l_all = row_groups_sum(l_run[rt]);
+        if (rt > 0) __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NO; c += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<vf4*>(ob + (wave * 16 + col) * OS + 16 * VE * (c / VE) + VE * (4 * g + i) + c % VE) =
+                    vf4{o[rt][c][i], o[rt][c + 1][i], o[rt][c + 2][i], o[rt][c + 3][i]};
+        if (g == 0) {
+            ml_s[wave][col][0] = m_run[rt];
+            ml_s[wave][col][1] = l_all;
+        }
+        __syncthreads();
+        for (int e = tid; e < 16 * (D / 4); e += 256) {
+            const int lr = e / (D / 4), dd = 4 * (e % (D / 4)), rr = 16 * rt + lr;
+            if (rr >= n_rows) continue;
+            float M = kNegInf;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, ml_s[w][lr][0]);
+            const float M_use = M == kNegInf ? 0.f : M;
+            float l = 0.f;
+            vf4 acc = vf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = fast_exp2(ml_s[w][lr][0] - M_use);
+                l += f * ml_s[w][lr][1];
+                acc += f * *reinterpret_cast<const vf4*>(ob + (w * 16 + lr) * OS + dd);
+            }
+            if (odd_s) {                 // values that are not finite, for the rows that see them
+                const int t = (row0 + rr) / p.G;
+                for (int key = max(k0, len); key < k1; ++key) {
+                    const int row = paged_row(pool, table, h, key);
+                    if (row < 0 || !sees(t, key - len)) continue;
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t at = row * (int64_t)pool.d + clamp_dim(dd + i);
+                        const float v = BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(vbase)[at] << 16)
+                                             : reinterpret_cast<const float*>(vbase)[at];
+                        if (not_finite(v)) acc[i] += v;
+                    }
+                }
+            }
+            if (live == 1) {
+                const int r = row0 + rr, t = r / p.G;
+                if (t >= count) continue;
+                float* out = p.o.p + b * p.o.sb + (h * p.G + r % p.G) * p.o.sh + t * p.o.st;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (FULL || dd + i < pool.d) out[(dd + i) * p.o.sd] = l == 0.f ? 0.f : acc[i] / l;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) store_coherent(rec + o_at + rr * D + dd + i, acc[i]);
+                if (dd == 0) {
+                    store_coherent(rec + 2 * rr, M);
+                    store_coherent(rec + 2 * rr + 1, l);
+                }
+            }
+        }
+    }
+    if (live == 1) return;
+
+    // ---- the last of the parts to arrive merges their records in order
+    wait_stores_performed();
+    __syncthreads();
+    uint32_t* const cnt = p.cnt + ((int64_t)bl * pool.Hkv + h) * p.n_rb + rb;
+    if (tid == 0)
+        last_s = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)live - 1;
+    __syncthreads();
+    if (!last_s) return;
+    if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int64_t step = heads_blocks * rec_floats;       // floats between two parts' records
+    const float* const first = p.ws + rec0 * rec_floats;
+    constexpr int NR = 8;                                 // records a thread has in flight
+    for (int e = tid; e < n_rows * (D / 4); e += 256) {
+        const int rr = e / (D / 4), dd = 4 * (e % (D / 4));
+        float M = kNegInf, l = 0.f;
+        vf4 acc = vf4{0.f, 0.f, 0.f, 0.f};
+        for (int c0 = 0; c0 < live; c0 += NR) {
+            float2 ml[NR];
+            vf4 x[NR];
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const float* at = first + min(c0 + c, live - 1) * step;
+                const __amdgpu_buffer_rsrc_t range = coherent_range(at, (uint32_t)rec_floats * 4u);
+                ml[c] = load_coherent2(range, (uint32_t)(8 * rr));
+                x[c] = load_coherent4(range, (uint32_t)(4 * (o_at + rr * D + dd)));
+            }
+            float M_new = M;
+#pragma unroll
+            for (int c = 0; c < NR; ++c) M_new = fmaxf(M_new, ml[c].x);
+            const float M_use = M_new == kNegInf ? 0.f : M_new;
+            const float old = fast_exp2(M - M_use);
+            l *= old;
+            acc *= old;
+            M = M_new;
+#pragma unroll
+            for (int c = 0; c < NR; ++c)
+                if (c0 + c < live) {
+                    const float f = fast_exp2(ml[c].x - M_use);
+                    l += f * ml[c].y;
+                    acc += f * x[c];
+                }
+        }
+        const int r = row0 + rr, t = r / p.G;
+        if (t >= count) continue;
+        float* out = p.o.p + b * p.o.sb + (h * p.G + r % p.G) * p.o.sh + t * p.o.st;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (FULL || dd + i < pool.d) out[(dd + i) * p.o.sd] = l == 0.f ? 0.f : acc[i] / l;
+    }
+}
+
+template <bool BF16, int D, int NRT, bool NT>
+hipError_t launch_tile(const PagedAttnParams& p, hipStream_t stream) {
+    const int64_t units = (int64_t)p.prefix[p.B] * p.pool.Hkv;
+    const int64_t wgs = p.n_rb > 1 ? (units + 7) / 8 * 8 * p.n_rb : units;
+    if (wgs > INT32_MAX) return hipErrorInvalidValue;
+    if (p.pool.d == D)
+        hipLaunchKernelGGL((paged_attention_kernel<BF16, D, NRT, true, NT>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((paged_attention_kernel<BF16, D, NRT, false, NT>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+
+template <bool BF16>
+hipError_t launch_type(const PagedAttnParams& p, hipStream_t stream) {
+    const int rows = paged_tile_rows(p.R, p.pool.d);
+    switch (paged_tile_dim(p.pool.d)) {
+    case 64:
+        return rows == 16 ? launch_tile<BF16, 64, 1, true>(p, stream)
+             : rows == 32 ? launch_tile<BF16, 64, 2, true>(p, stream)
+                          : launch_tile<BF16, 64, 4, false>(p, stream);
+    case 128:
+        return rows == 16 ? launch_tile<BF16, 128, 1, true>(p, stream)
+             : rows == 32 ? launch_tile<BF16, 128, 2, true>(p, stream)
+                          : launch_tile<BF16, 128, 4, false>(p, stream);
+    default:
+        return rows == 16 ? launch_tile<BF16, 256, 1, true>(p, stream)
+                          : launch_tile<BF16, 256, 2, false>(p, stream);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_paged_attention(const PagedAttnParams& p, hipStream_t stream) {
+    if (p.B <= 0 || p.R <= 0) return hipSuccess;
+    return p.pool.bf16 ? launch_type<true>(p, stream) : launch_type<false>(p, stream);
+}
+
+}  // namespace nne

@@ -26,7 +26,7 @@ struct Args {
     PyObject* const* a;
     Py_ssize_t n, i = 0;
     bool ok = true;
-    Py_buffer host[1];
+    Py_buffer host[2];
     int n_host = 0;
 
     Args(PyObject* const* args, Py_ssize_t count) : a(args), n(count) {}
@@ -245,9 +245,109 @@ PyObject* qkv_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return PyLong_FromLong(rc);
 }
 
+PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n);
+    auto* f = function<decltype(nne_qk_norm_rope)>(a);
+    auto* q = a.pointer<const float>();
+    const auto qs = a.dims(), qst = a.dims();
+    auto* qo = a.pointer<float>();
+    const auto qot = a.dims();
+    auto* k = a.pointer<const float>();
+    const auto ks = a.dims(), kst = a.dims();
+    auto* ko = a.pointer<float>();
+    const auto kot = a.dims();
+    auto *qw = a.pointer<const float>(), *kw = a.pointer<const float>();
+    const int has_norm = (int)a.integer();
+    const float eps = a.real();
+    auto *cos = a.pointer<const float>(), *sin = a.pointer<const float>();
+    const int64_t max_seq = a.integer(), table_d = a.integer();
+    auto* start = a.pointer<const int32_t>();
+    const int32_t* start_host = a.host_array();
+    auto* depths = a.pointer<const int32_t>();
+    const int32_t* depths_host = a.host_array();
+    void* stream = a.pointer<void>();
+    if (!a.done()) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f(q, qs.v, qst.v, qo, qot.v, k, ks.v, kst.v, ko, kot.v, qw, kw, has_norm, eps, cos, sin, max_seq, table_d,
+           start, start_host, depths, depths_host, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n);
+    auto* f = function<decltype(nne_paged_append)>(a);
+    auto* cache = a.pointer<const nne_paged_cache_t>();
+    auto* k = a.pointer<const float>();
+    const auto kst = a.dims();
+    auto* v = a.pointer<const float>();
+    const auto vst = a.dims();
+    const int64_t T = a.integer();
+    auto* counts = a.pointer<const int32_t>();
+    const int32_t* counts_host = a.host_array();
+    auto* depths = a.pointer<const int32_t>();
+    const int32_t* depths_host = a.host_array();
+    auto *cos = a.pointer<const float>(), *sin = a.pointer<const float>();
+    const int64_t max_seq = a.integer(), table_d = a.integer();
+    void* stream = a.pointer<void>();
+    if (!a.done()) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f(cache, k, kst.v, v, vst.v, T, counts, counts_host, depths, depths_host, cos, sin, max_seq, table_d, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n);
+    auto* f = function<decltype(nne_paged_attention)>(a);
+    auto* cache = a.pointer<const nne_paged_cache_t>();
+    auto* q = a.pointer<const float>();
+    const auto qst = a.dims();
+    auto* o = a.pointer<float>();
+    const auto ost = a.dims();
+    const int64_t Hq = a.integer(), T = a.integer();
+    auto* counts = a.pointer<const int32_t>();
+    const int32_t* counts_host = a.host_array();
+    auto* parents = a.pointer<const int32_t>();
+    const int32_t* parents_host = a.host_array();
+    const int has_scale = (int)a.integer();
+    const float scale = a.real();
+    const nne_workspace_t* ws = a.workspace();
+    void* stream = a.pointer<void>();
+    if (!a.done()) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f(cache, q, qst.v, o, ost.v, Hq, T, counts, counts_host, parents, parents_host, has_scale, scale, ws, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+PyObject* paged_commit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Args a(args, n);
+    auto* f = function<decltype(nne_paged_commit)>(a);
+    auto* cache = a.pointer<const nne_paged_cache_t>();
+    const int64_t layers = a.integer(), stride = a.integer();
+    auto* counts = a.pointer<const int32_t>();
+    const int32_t* counts_host = a.host_array();
+    auto* paths = a.pointer<const int32_t>();
+    const int32_t* paths_host = a.host_array();
+    const int64_t J = a.integer();
+    const nne_workspace_t* ws = a.workspace();
+    void* stream = a.pointer<void>();
+    if (!a.done()) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f(cache, layers, stride, counts, counts_host, paths, paths_host, J, ws, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 #define NNE_METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {NNE_METHOD(flash), NNE_METHOD(attention), NNE_METHOD(decode_attention),
-                         NNE_METHOD(decode_step), NNE_METHOD(qkv_rope), {nullptr, nullptr, 0, nullptr}};
+                         NNE_METHOD(decode_step), NNE_METHOD(qkv_rope), NNE_METHOD(qk_norm_rope),
+                         NNE_METHOD(paged_append), NNE_METHOD(paged_attention), NNE_METHOD(paged_commit), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "nne_pycall", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
