@@ -762,43 +762,55 @@ def qkv_rope(x, w_packed, bq, bk, bv, rope, pos_dev, pos_host, num_heads, num_kv
     return q_out, k_out, v_out
 
 
-def _on_device(device, *ts):
-    """The tensors are on ``device``, and it is the current one (whose streams
-    the calls run on)."""
-    import torch
+_torch = None
+
+
+def _check_f32(index, *ts):
+    """float32 tensors on GPU ``index``, and that is the current one (whose streams
+    the calls run on).  (The checks of a small call's tensors: a device object and
+    an import statement cost more than the rest of them.)"""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    f32 = _torch.float32
     for t in ts:
-        if t.device != device:
-            raise InvalidArgument("Invalid configuration or argument: expected tensors on %s, got %s"
-                                  % (device, t.device))
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise InvalidArgument("Invalid configuration or argument: %s is not the current device"
-                              % device)
+        if t.dtype is not f32 or t.get_device() != index or index < 0:
+            raise InvalidArgument("Invalid configuration or argument: expected float32 tensors on GPU "
+                                  "%d, got %s on %s" % (index, t.dtype, t.device))
+    if _torch._C._cuda_getDevice() != index:
+        raise InvalidArgument("Invalid configuration or argument: GPU %d is not the current device"
+                              % index)
+
+
+def _stream_on(index, stream):
+    return _torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
 
 
 def _new_like(t, stream):
-    """An uninitialised contiguous tensor of t's shape, allocated for the stream
-    that writes it."""
-    import torch
+    """An uninitialised tensor of t's shape and order of dims, allocated for the
+    stream that writes it."""
     if stream is None:
-        return t.new_empty(t.shape)
-    with torch.cuda.stream(stream):
-        return t.new_empty(t.shape)
+        return _torch.empty_like(t)
+    with _torch.cuda.stream(stream):
+        return _torch.empty_like(t)
 
 
 def _int_array(x, shape, what):
-    a = np.ascontiguousarray(x, dtype=np.int32)
+    a = x
+    if type(a) is not np.ndarray or a.dtype != np.int32 or not a.flags.c_contiguous:
+        a = np.ascontiguousarray(x, dtype=np.int32)
     if a.shape != shape:
         raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s (%s)"
                             % (list(shape), list(a.shape), what))
     return a
 
 
-def _check_int_dev(t, shape, device, what):
-    import torch
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+def _check_int_dev(t, shape, index, what):
+    if t.dtype is not _torch.int32 or t.get_device() != index or t.shape != shape or \
+            not t.is_contiguous():
         raise InvalidArgument("Invalid configuration or argument: %s must be a contiguous int32 "
-                              "tensor of shape %s" % (what, list(shape)))
-    _on_device(device, t)
+                              "tensor of shape %s on GPU %d" % (what, list(shape), index))
 
 
 class DraftTree:
@@ -826,6 +838,8 @@ class DraftTree:
             depths[:, i] = np.where(p < 0, 0, depths[np.arange(b), np.maximum(p, 0)] + 1)
         self.parents_host, self.parents_dev = parents, self._dev(parents)
         self.depths_host, self.depths_dev = depths, self._dev(depths)
+        self._parents = self._pair(self.parents_dev, parents)
+        self._depths = self._pair(self.depths_dev, depths)
 
     @classmethod
     def chain(cls, batch, tokens, counts=None, device="cuda"):
@@ -834,6 +848,7 @@ class DraftTree:
         self = cls.__new__(cls)
         self._set((int(batch), int(tokens)), counts, device)
         self.parents_host = self.parents_dev = self.depths_host = self.depths_dev = None
+        self._parents = self._depths = _NO_PAIR
         return self
 
     def _dev(self, a):
@@ -851,36 +866,42 @@ class DraftTree:
                 raise InvalidArgument("Invalid configuration or argument: counts outside [0, %d]"
                                       % self.tokens)
             self.counts_dev = self._dev(self.counts_host)
+        self._counts = self._pair(self.counts_dev, self.counts_host)
+        self._index = -1 if self.device.index is None else self.device.index
 
     @staticmethod
     def _pair(dev, host):
         return (None if dev is None else dev.data_ptr(), host)
 
-    def _check(self, batch, tokens, device):
-        if (self.batch, self.tokens) != (batch, tokens):
+    def _check(self, batch, tokens, index):
+        if self.batch != batch or self.tokens != tokens:
             raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
                                 % ([self.batch, self.tokens], [batch, tokens]))
-        if self.device != device:
-            raise InvalidArgument("Invalid configuration or argument: expected tensors on %s, got %s"
-                                  % (device, self.device))
-
-    def _counts(self):
-        return self._pair(self.counts_dev, self.counts_host)
-
-    def _parents(self):
-        return self._pair(self.parents_dev, self.parents_host)
-
-    def _depths(self):
-        return self._pair(self.depths_dev, self.depths_host)
+        if self._index != index:
+            raise InvalidArgument("Invalid configuration or argument: the draft is on %s, not on GPU %d"
+                                  % (self.device, index))
 
 
 _NO_PAIR = (None, None)
 _NO_ROPE = (None, None, 0, 0)
+_NO_K = (None, (0, 0, 0, 0), (0, 0, 0, 0), None, (0, 0, 0, 0))
 
 
-def _rope_args(rope):
-    return _NO_ROPE if rope is None else (rope.cos.data_ptr(), rope.sin.data_ptr(),
-                                          rope.max_seq_len, rope.head_dim)
+def _rope_args(rope, index):
+    if rope is None:
+        return _NO_ROPE
+    cos, sin = rope.cos, rope.sin
+    if cos.get_device() != index or sin.get_device() != index:
+        raise InvalidArgument("Invalid configuration or argument: the rotary tables are on %s, not on "
+                              "GPU %d" % (cos.device, index))
+    return cos.data_ptr(), sin.data_ptr(), rope.max_seq_len, rope.head_dim
+
+
+def _check_out(out, shape, index):
+    _check_f32(index, out)
+    if out.shape != shape:
+        raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                            % (list(shape), list(out.shape)))
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6, draft=None,
@@ -891,44 +912,47 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6
     start[b] + t, or with a ``draft`` at start[b] + its depth in the tree
     (``start``: int32 [B], device and host copies).  Weights are [d] or None (ones);
     rope=None: no rotation; eps=None: no norm, the rotation alone (no weights);
-    k=None: q alone.  Returns (q_out, k_out): new contiguous tensors by default, or
-    the given ones (q and k themselves are fine)."""
-    _shape4(q, "Q")
-    tensors = [t for t in (q, k, q_weight, k_weight, q_out, k_out) if t is not None]
-    _require_f32_cuda(*tensors)
-    _on_device(q.device, *tensors)
-    b, _, t, d = q.shape
+    k=None: q alone.  Returns (q_out, k_out): new tensors in the inputs' order of dims
+    by default, or the given ones (q and k themselves are fine)."""
+    qs, qst = _shape4(q, "Q")
+    index = q.get_device()
+    _check_f32(index, q)
+    b, _, t, d = qs
     for w in (q_weight, k_weight):
-        if w is not None and (tuple(w.shape) != (d,) or not w.is_contiguous()):
-            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
-                                % ([d], list(w.shape)))
-    if k is not None:
-        _shape4(k, "K")
-    for x, out in ((q, q_out), (k, k_out)):
-        if out is not None and (x is None or out.shape != x.shape):
-            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
-                                % ([] if x is None else list(x.shape), list(out.shape)))
+        if w is not None:
+            _check_f32(index, w)
+            if w.shape != (d,) or not w.is_contiguous():
+                raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                    % ([d], list(w.shape)))
     if q_out is None:
         q_out = _new_like(q, stream)
-    if k is not None and k_out is None:
-        k_out = _new_like(k, stream)
+    else:
+        _check_out(q_out, qs, index)
+    ks = _NO_K
+    if k is not None:
+        _check_f32(index, k)
+        kshape, kst = _shape4(k, "K")
+        if k_out is None:
+            k_out = _new_like(k, stream)
+        else:
+            _check_out(k_out, kshape, index)
+        ks = (k.data_ptr(), kshape, kst, k_out.data_ptr(), k_out.stride())
+    elif k_out is not None:
+        raise InvalidArgument("Invalid configuration or argument: k_out without k")
     start, depths = _NO_PAIR, _NO_PAIR
     if rope is not None:
         start_host = _int_array(start_host, (b,), "start_host")
-        _check_int_dev(start_dev, (b,), q.device, "start_dev")
-        _on_device(q.device, rope.cos, rope.sin)
+        _check_int_dev(start_dev, (b,), index, "start_dev")
         start = (start_dev.data_ptr(), start_host)
         if draft is not None:
-            draft._check(b, t, q.device)
-            depths = draft._depths()
-    ks = (None, (0, 0, 0, 0), (0, 0, 0, 0), None, (0, 0, 0, 0))
-    if k is not None:
-        ks = (k.data_ptr(), k.shape, k.stride(), k_out.data_ptr(), k_out.stride())
+            draft._check(b, t, index)
+            depths = draft._depths
     check(_native().qk_norm_rope(
-        q.data_ptr(), q.shape, q.stride(), q_out.data_ptr(), q_out.stride(), *ks,
+        q.data_ptr(), qs, qst, q_out.data_ptr(), q_out.stride(), *ks,
         None if q_weight is None else q_weight.data_ptr(),
         None if k_weight is None else k_weight.data_ptr(), eps is not None,
-        float(eps or 0.0), *_rope_args(rope), *start, *depths, _stream(stream)))
+        0.0 if eps is None else eps, *_rope_args(rope, index), *start, *depths,
+        _stream_on(index, stream)))
     return q_out, k_out
 
 
@@ -941,11 +965,13 @@ class _StepWorkspace(Workspace):
         super().__init__(device)
         self._kept = []
 
+    def grows(self, size):
+        return size.records_bytes > (0 if self.records is None else self.records.numel()) or \
+            size.n_counters > (0 if self.counters is None else self.counters.numel())
+
     def reserve(self, size, stream=None):
         import torch
-        have = (0 if self.records is None else self.records.numel(),
-                0 if self.counters is None else self.counters.numel())
-        if size.records_bytes <= have[0] and size.n_counters <= have[1]:
+        if not self.grows(size):
             return self
         if torch.cuda.is_current_stream_capturing():
             raise InvalidArgument("Invalid configuration or argument: the workspace cannot grow "
@@ -990,13 +1016,14 @@ class PagedKVCache:
         self._k = torch.zeros(shape, dtype=self.dtype, device=device)
         self._v = torch.zeros(shape, dtype=self.dtype, device=device)
         self._device = self._k.device
+        self._index = self._k.get_device()
         self.table_host = np.full((self.batch, self.max_pages), -1, np.int32)
         self.table_dev = torch.full((self.batch, self.max_pages), -1, dtype=torch.int32,
                                     device=device)
         self.lens_host = np.zeros(self.batch, np.int32)
         self.lens_dev = torch.zeros(self.batch, dtype=torch.int32, device=device)
         self._ws = _StepWorkspace(self._device)
-        self._sizes = {}
+        self._sizes, self._ws_ready = {}, {}
         self._bind()
 
     @property
@@ -1122,69 +1149,74 @@ class PagedKVCache:
         key = (num_heads, tokens)
         if key not in self._sizes:
             size = NneWorkspaceSize()
-            s = NnePagedCache.from_buffer_copy(self._structs[0][1]) if self._structs else None
-            check(lib().nne_paged_workspace_size(None if s is None else ctypes.addressof(s),
+            check(lib().nne_paged_workspace_size(self._addr[0][1] if self._addr else None,
                                                  num_heads, tokens, ctypes.byref(size)))
             self._sizes[key] = size
         return self._sizes[key]
 
+    def _ws_args(self, num_heads, tokens, stream):
+        """The workspace of a step, as the native calls take it."""
+        args = self._ws_ready.get((num_heads, tokens))
+        if args is None:
+            size = self._size(num_heads, tokens) if tokens else NneWorkspaceSize(0, self.batch)
+            if self._ws.grows(size):
+                self._ws_ready.clear()
+            args = self._ws_ready[num_heads, tokens] = _ws_arg(self._ws, size, stream)
+        return args
+
     def reserve_workspace(self, num_heads, tokens, stream=None):
         """Grows the cache's workspace to steps of ``tokens`` tokens and
         ``num_heads`` query heads, as a step under capture needs it to be."""
-        self._ws.reserve(self._size(int(num_heads), int(tokens)), stream)
+        self._ws_args(int(num_heads), int(tokens), stream)
 
     def append(self, layer_idx, k_new, v_new, rope=None, draft=None, stream=None):
         """Writes the rows of new tokens, k_new / v_new [B, Hkv, T, d] (any
         strides), behind the counted rows, the keys rotated at their tokens'
         positions (``rope``: a RotaryEmbedding; None: as they are)."""
         self._check_layer(layer_idx)
-        _require_f32_cuda(k_new, v_new)
-        _on_device(self._device, k_new, v_new)
-        _shape4(k_new, "K")
-        b, h, t, d = k_new.shape
-        if (b, h, d) != (self.batch, self.num_kv_heads, self.head_dim) or v_new.shape != k_new.shape:
+        index = self._index
+        _check_f32(index, k_new, v_new)
+        shape, kst = _shape4(k_new, "K")
+        b, h, t, d = shape
+        if b != self.batch or h != self.num_kv_heads or d != self.head_dim or v_new.shape != shape:
             raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s" % (
                 [self.batch, self.num_kv_heads, t, self.head_dim],
-                list(v_new.shape if v_new.shape != k_new.shape else k_new.shape)))
+                list(v_new.shape if v_new.shape != shape else shape)))
         counts = depths = _NO_PAIR
         if draft is not None:
-            draft._check(b, t, self._device)
-            counts, depths = draft._counts(), draft._depths()
-        if rope is not None:
-            _on_device(self._device, rope.cos, rope.sin)
+            draft._check(b, t, index)
+            counts, depths = draft._counts, draft._depths
         check(_native().paged_append(
-            self._addr[layer_idx][0], k_new.data_ptr(), k_new.stride(), v_new.data_ptr(),
-            v_new.stride(), t, *counts, *depths, *_rope_args(rope), _stream(stream)))
+            self._addr[layer_idx][0], k_new.data_ptr(), kst, v_new.data_ptr(), v_new.stride(), t,
+            *counts, *depths, *_rope_args(rope, index), _stream_on(index, stream)))
 
     def attend(self, layer_idx, q, draft=None, out=None, scale=None, stream=None):
         """Attention of the appended tokens' queries q [B, Hq, T, d] over the
-        counted rows and those new ones that lead to them.  Rows of ``out`` for
-        tokens past a draft's counts are left as they were (undefined in a new
-        ``out``)."""
+        counted rows and those new ones that lead to them.  Rows of ``out`` (by
+        default a new tensor in q's order of dims) for tokens past a draft's counts
+        are left as they were."""
         self._check_layer(layer_idx)
-        _shape4(q, "Q")
-        _require_f32_cuda(q)
-        _on_device(self._device, q)
-        b, hq, t, d = q.shape
-        if (b, d) != (self.batch, self.head_dim) or hq == 0 or hq % self.num_kv_heads != 0:
+        index = self._index
+        _check_f32(index, q)
+        shape, qst = _shape4(q, "Q")
+        b, hq, t, d = shape
+        if b != self.batch or d != self.head_dim or hq == 0 or hq % self.num_kv_heads != 0:
             raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s" % (
-                [self.batch, self.num_kv_heads, t, self.head_dim], list(q.shape)))
+                [self.batch, self.num_kv_heads, t, self.head_dim], list(shape)))
         if out is None:
             out = _new_like(q, stream)
         else:
-            _require_f32_cuda(out)
-            _on_device(self._device, out)
-            if out.shape != q.shape:
-                raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
-                                    % (list(q.shape), list(out.shape)))
+            _check_out(out, shape, index)
         counts = parents = _NO_PAIR
         if draft is not None:
-            draft._check(b, t, self._device)
-            counts, parents = draft._counts(), draft._parents()
+            draft._check(b, t, index)
+            counts, parents = draft._counts, draft._parents
+        if t == 0:
+            return out
         check(_native().paged_attention(
-            self._addr[layer_idx][1], q.data_ptr(), q.stride(), out.data_ptr(), out.stride(), hq, t,
-            *counts, *parents, scale is not None, float(scale or 0.0),
-            _ws_arg(self._ws, self._size(hq, t), stream), _stream(stream)))
+            self._addr[layer_idx][1], q.data_ptr(), qst, out.data_ptr(), out.stride(), hq, t,
+            *counts, *parents, scale is not None, 0.0 if scale is None else scale,
+            self._ws_args(hq, t, stream), _stream_on(index, stream)))
         return out
 
     def commit(self, counts, counts_host=None, paths=None, paths_host=None, stream=None):
@@ -1192,23 +1224,25 @@ class PagedKVCache:
         first ``counts`` tokens), or int32 [B] on the device with its host copy.
         paths (int32 [B, J], device and host copies): the accepted tokens of a
         tree, ascending; their rows move behind the counted ones."""
+        index, batch = self._index, self.batch
+        _check_f32(index)
         if isinstance(counts, (int, np.integer)):
-            host = np.full(self.batch, counts, np.int32)
-            dev = None
+            host, dev = np.full(batch, counts, np.int32), None
         else:
-            _check_int_dev(counts, (self.batch,), self._device, "counts")
-            host = _int_array(counts_host, (self.batch,), "counts_host")
-            dev = counts.data_ptr()
-        j, path = int(host.max()) if self.batch else 0, _NO_PAIR
+            _check_int_dev(counts, (batch,), index, "counts")
+            host, dev = _int_array(counts_host, (batch,), "counts_host"), counts.data_ptr()
+        path = _NO_PAIR
         if paths is not None:
-            j = int(paths.shape[-1])
-            _check_int_dev(paths, (self.batch, j), self._device, "paths")
-            path = (paths.data_ptr(), _int_array(paths_host, (self.batch, j), "paths_host"))
+            j = paths.shape[-1]
+            _check_int_dev(paths, (batch, j), index, "paths")
+            path = (paths.data_ptr(), _int_array(paths_host, (batch, j), "paths_host"))
+        else:
+            j = int(host.max()) if batch else 0
         if not self._addr:
             raise InvalidArgument("Invalid configuration or argument: a cache of no layers")
         check(_native().paged_commit(
             self._addr[0][0], self._shape[0], self._layer_stride, dev, host, *path, max(j, 0),
-            _ws_arg(self._ws, NneWorkspaceSize(0, self.batch), stream), _stream(stream)))
+            self._ws_args(0, 0, stream), _stream_on(index, stream)))
 
 
 class GroupedQueryAttention:

@@ -114,7 +114,7 @@ nne::PagedPool make_pool(const nne_paged_cache_t* c) {
     p.max_pages = (int)c->max_pages;
     p.table = c->table;
     p.lens = c->lens_dev;
-    nne::paged_division(p);
+    p.by_page = nne::divisor(c->page_size);
     return p;
 }
 
@@ -153,8 +153,8 @@ int check_positions(const int32_t* start, const int32_t* depths_dev, const int32
 }
 
 // Workgroups of a part, per KV head of the cache.
-int64_t row_blocks(int64_t R, int64_t d) {
-    const int tile = nne::paged_tile_rows((int)std::min<int64_t>(R, 1 << 20), (int)d);
+int64_t row_blocks(int64_t R) {
+    const int tile = nne::paged_tile_rows((int)R);
     return (R + tile - 1) / tile;
 }
 
@@ -167,14 +167,17 @@ int check_attention_heads(const nne_paged_cache_t* c, int64_t Hq, int64_t T) {
     return NNE_OK;
 }
 
+// Workspace of launches over the batch's groups of sequences, with T tokens.
 nne_workspace_size_t attention_size(const nne_paged_cache_t* c, int64_t Hq, int64_t T) {
-    const int64_t R = Hq / c->Hkv * T, n_rb = row_blocks(R, c->d);
-    const int64_t B = std::min<int64_t>(c->B, nne::kPagedSeqs);
-    const int tile = nne::paged_tile_rows((int)std::min<int64_t>(R, 1 << 20), (int)c->d);
-    const int64_t rec = 4 * nne::paged_record_floats((int)std::min<int64_t>(R, tile), nne::paged_tile_dim((int)c->d));
+    const int64_t R = Hq / c->Hkv * T, units = c->Hkv * row_blocks(R);
+    const int64_t rec = 4 * nne::paged_record_floats((int)std::min<int64_t>(R, nne::paged_tile_rows((int)R)),
+                                                     nne::paged_tile_dim((int)c->d));
+    const int64_t group = std::min<int64_t>(c->B, nne::kPagedSeqs), rest = c->B % nne::kPagedSeqs;
+    const int cus = nne::cus_of_device();
     nne_workspace_size_t s;
-    s.records_bytes = (uint64_t)(nne::paged_max_records(B, c->Hkv * n_rb, nne::cus_of_device()) * rec);
-    s.n_counters = (uint64_t)std::max<int64_t>(B * c->Hkv * n_rb, c->B);
+    s.records_bytes = (uint64_t)(rec * std::max(nne::paged_max_records(group, units, rec, cus),
+                                                rest ? nne::paged_max_records(rest, units, rec, cus) : 0));
+    s.n_counters = (uint64_t)std::max<int64_t>(group * units, c->B);
     return s;
 }
 
@@ -313,7 +316,16 @@ int nne_paged_workspace_size(const nne_paged_cache_t* cache, int64_t Hq, int64_t
     if (rc == NNE_OK) rc = check_attention_heads(cache, Hq, T);
     if (rc) return rc;
     if (cache->B == 0 || T == 0) return NNE_OK;
-    *out = attention_size(cache, Hq, T);   // grows with T: fewer tokens need no more
+    // Records grow with the tokens up to where launches no longer split: the most
+    // that a step of T tokens or fewer needs is at the last that does.
+    *out = attention_size(cache, Hq, T);
+    for (int64_t lo = 1, hi = T; lo <= hi;) {
+        const int64_t t = lo + (hi - lo) / 2;
+        const nne_workspace_size_t s = attention_size(cache, Hq, t);
+        out->records_bytes = std::max(out->records_bytes, s.records_bytes);
+        if (s.records_bytes) lo = t + 1;
+        else hi = t - 1;
+    }
     return NNE_OK;
 }
 
@@ -353,13 +365,17 @@ int nne_paged_attention(const nne_paged_cache_t* cache, const float* q, const in
     p.pool = make_pool(cache);
     p.counts = counts_dev;
     p.parents = parents_dev;
-    p.Hq = (int)Hq;
     p.G = (int)(Hq / cache->Hkv);
     p.T = (int)T;
     p.R = p.G * p.T;
-    p.n_rb = (int)row_blocks(p.R, d);
-    p.rec_rows = std::min(p.R, nne::paged_tile_rows(p.R, (int)d));
+    p.tile_rows = nne::paged_tile_rows(p.R);
+    p.n_rb = (int)row_blocks(p.R);
+    p.by_g = nne::divisor(p.G);
+    p.by_hkv = nne::divisor(p.pool.Hkv);
+    p.by_rb = nne::divisor(p.n_rb);
+    p.rec_rows = std::min(p.R, p.tile_rows);
     p.vec_q = vec_view(q, qs.v);
+    p.vec_o = vec_view(o, os.v);
     p.qscale = (has_scale ? scale : 1.0f / std::sqrt((float)d)) * nne::kLog2e;
     const int64_t rec_bytes = 4 * nne::paged_record_floats(p.rec_rows, nne::paged_tile_dim((int)d));
     const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -1,10 +1,10 @@
 // Attention over a paged KV cache: a step's new tokens -- one, a chain, or a
 // tree -- against their sequence's rows and the new ones on their path.
 //
-//   o[r] = sum_c 2^(s[r,c] - m[r]) v[c] / sum_c 2^(s[r,c] - m[r]),
+//   o[r] = sum_c 2^(s[r,c] - m[r]) v[c] / sum_c 2^(s[r,c] - m[r]),   any m[r],
 //   s[r,c] = (scale log2(e) q[r]) . k[c] where r sees c, else -inf,
 //
-// in one pass over the keys with the running maximum m and sum per row.
+// in one pass over the keys, with m[r] kept above the scores seen so far.
 //
 // A KV head's G * T query rows (row r: token r / G of query head r % G) are the
 // columns of MFMA tiles, its keys the rows:  S^T = K Q^T, O^T += V^T P^T.  Both
@@ -25,6 +25,7 @@
 // the last workgroup to arrive merges in the order of the parts, so results do
 // not depend on who that is.
 #include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "paged_device.hpp"
@@ -39,7 +40,12 @@ typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
-constexpr int kStage = 2048;     // keys whose pool rows are in LDS at a time
+constexpr int kStage = 1024;     // keys whose pool rows are in LDS at a time
+constexpr int kTable = 512;      // pages of a sequence whose table row goes to LDS whole
+// A row's weights are taken relative to 2^8 times the largest so far (they cancel
+// in the quotient), so that a larger one changes nothing until it passes that:
+// nearly every block skips the scaling of O, and no weight is above 1.
+constexpr float kSlack = 8.f;
 
 __device__ __forceinline__ float row_groups_max(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -63,6 +69,14 @@ __device__ __forceinline__ V load_vec(const void* p) {
     else return *static_cast<const V*>(p);
 }
 
+// 16- and 8-byte forms of store_coherent (buffer stores with the same policy).
+__device__ __forceinline__ void store_coherent4(__amdgpu_buffer_rsrc_t range, uint32_t byte_offset, vf4 x) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, x), range, byte_offset, 0, 16);
+}
+__device__ __forceinline__ void store_coherent2(__amdgpu_buffer_rsrc_t range, uint32_t byte_offset, float x, float y) {
+    __builtin_amdgcn_raw_buffer_store_b64(uintx2{__float_as_uint(x), __float_as_uint(y)}, range, byte_offset, 0, 16);
+}
+
 // What differs between the pools' types.  KB: keys of a block, JN: keys of a
 // block per lane, VE: consecutive dims of a V load.
 template <bool BF16, int D>
@@ -75,6 +89,7 @@ struct Shape {
     static constexpr int KS = BF16 ? D / 32 : D / 16; // K loads per tile
     static constexpr int NO = D / 16;                 // 16-dim tiles of O
     static constexpr int ES = BF16 ? 2 : 4;           // bytes of an element
+    static constexpr int QP = BF16 ? 3 : 1;           // parts of Q
 };
 
 // Key of a block that slot j of lane group g stands for.
@@ -90,39 +105,49 @@ __device__ __forceinline__ bool not_finite(float x) {
 // BF16: the pools' type.  D: dims, padded.  NRT: 16-row tiles of query rows.
 // FULL: d == D.  NT: no other workgroup reads these keys.
 template <bool BF16, int D, int NRT, bool FULL, bool NT>
-__global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_attention_kernel(const PagedAttnParams p) {
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(const PagedAttnParams p) {
     using S = Shape<BF16, D>;
     constexpr int KB = S::KB, JN = S::JN, VE = S::VE, NV = S::NV, KT = S::KT, KS = S::KS, NO = S::NO;
     constexpr int OS = D + 4;                        // row stride of the merge buffer
     constexpr int ROWS = 16 * NRT;
 
-    __shared__ __attribute__((aligned(16))) float ob[4 * 16 * OS];
+    // Q^T in operand order, [row tile][step][part][lane], until the last block;
+    // then the waves' O.
+    constexpr int QN = NRT * KS * S::QP * 64;
+    constexpr int ON = 4 * 16 * OS / 4;
+    __shared__ uintx4 smem[QN > ON ? QN : ON];
+    float* const ob = reinterpret_cast<float*>(smem);
     __shared__ __attribute__((aligned(16))) int rows_s[kStage];
     __shared__ float ml_s[4][16][2];
     __shared__ uint32_t anc_s[kPagedTreeNodes][kPagedTreeNodes / 32];
     __shared__ int nxt_s[kPagedTreeNodes];
+    __shared__ int table_s[kTable];
     __shared__ int last_s, odd_s;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const PagedPool& pool = p.pool;
+    // Everything up to the first K and V is latency: one trip for the arguments,
+    // one for the length, the page table and Q together, one for K and V.
+    const int pref_lo = p.prefix[min(lane + 1, kPagedSeqs)], pref_hi = p.prefix[min(lane + 65, kPagedSeqs)];
+    warm_kernargs<0, sizeof(PagedAttnParams)>();
+    asm volatile("" ::"v"(pref_lo), "v"(pref_hi));
 
     // Workgroup -> (part and KV head, row block).  With several row blocks, the
     // ones that read the same keys follow each other on one XCD (workgroups go to
     // the 8 XCDs in turn), whose L2 then serves them.
     int unit = blockIdx.x, rb = 0;
     if (p.n_rb > 1) {
-        const int x = unit & 7, y = unit >> 3;
-        rb = y % p.n_rb;
-        unit = (y / p.n_rb) * 8 + x;
+        const int x = unit & 7, y = unit >> 3, z = quotient(y, p.by_rb);
+        rb = y - z * p.n_rb;
+        unit = z * 8 + x;
     }
     if (unit >= p.prefix[p.B] * pool.Hkv) return;
-    const int part_all = unit / pool.Hkv, h = unit % pool.Hkv;
+    const int part_all = quotient(unit, p.by_hkv), h = unit - part_all * pool.Hkv;
     int bl;
     {
-        const int lo = lane < p.B ? p.prefix[lane + 1] : INT32_MAX;
-        const int hi = lane + 64 < p.B ? p.prefix[lane + 65] : INT32_MAX;
+        const int lo = lane < p.B ? pref_lo : INT32_MAX, hi = lane + 64 < p.B ? pref_hi : INT32_MAX;
         bl = __popcll(__builtin_amdgcn_ballot_w64(lo <= part_all)) +
              __popcll(__builtin_amdgcn_ballot_w64(hi <= part_all));
     }
@@ -131,50 +156,78 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
 
     const int row0 = rb * ROWS;
     const int n_rows = min(ROWS, p.R - row0);
-    const int len = paged_len(pool, b);
+    const int raw_len = pool.lens[b];
     const int count = paged_count(p.counts, b, p.T);
-    if (row0 / p.G >= count) return;                 // no token of this block exists
-    // Keys that some row sees, cut into equal parts of whole 32-key steps.
-    const int seen = p.parents ? count : min(count, (row0 + n_rows - 1) / p.G + 1);
-    const int n_keys = len + seen;
-    const int part_len = ((n_keys + n_parts - 1) / n_parts + 31) & ~31;
-    const int k0 = part * part_len, k1 = min(n_keys, k0 + part_len);
-    if (k0 >= k1) return;                            // part 0 always has keys
-    const int live = (n_keys + part_len - 1) / part_len;
+    const int32_t* const table = pool.table + (int64_t)b * pool.max_pages;
+    const bool table_fits = pool.max_pages <= kTable;
+    int page[kTable / 256];
+#pragma unroll
+    for (int i = 0; i < kTable / 256; ++i)
+        page[i] = table_fits && tid + 256 * i < pool.max_pages ? table[tid + 256 * i] : -1;
 
-    // Q^T: the second operand of S^T, scaled; row col of tile rt.
-    uintx4 qb[BF16 ? NRT : 1][BF16 ? KS : 1][3];
-    vf4 qf[BF16 ? 1 : NRT][BF16 ? 1 : KS];
-    int tok[NRT];
+    // Q^T, the second operand of S^T, scaled: 4 or 8 dims of a row per thread and
+    // turn, every load issued before the first use.
+    constexpr int QT = (NRT * KS * 64 + 255) / 256;
+    vf4 qx[QT][BF16 ? 2 : 1];
 #pragma unroll
-    for (int rt = 0; rt < NRT; ++rt) {
-        const int r = min(row0 + 16 * rt + col, p.R - 1);
-        const bool rok = 16 * rt + col < n_rows;
-        tok[rt] = r / p.G;
-        const float* qp = p.q.p + b * p.q.sb + (h * p.G + r % p.G) * p.q.sh + tok[rt] * p.q.st;
-        auto dims4 = [&](int c) __attribute__((always_inline)) {
+    for (int i = 0; i < QT; ++i) {
+        const int e = tid + 256 * i, qc = e & 15, qg = (e >> 4) & 3, st = (e >> 6) % KS, rt = (e >> 6) / KS;
+        const bool rok = rt < NRT && 16 * rt + qc < n_rows;
+        const int r = rok ? row0 + 16 * rt + qc : row0, t = quotient(r, p.by_g);
+        const float* const qp = p.q.p + b * p.q.sb + (h * p.G + r - t * p.G) * p.q.sh + t * p.q.st;
+#pragma unroll
+        for (int y = 0; y < (BF16 ? 2 : 1); ++y) {
+            const int c = BF16 ? 32 * st + 8 * qg + 4 * y : 16 * st + 4 * qg;
             vf4 x = vf4{0.f, 0.f, 0.f, 0.f};
-            if (rok && (FULL || c < pool.d))
-                x = p.vec_q ? *reinterpret_cast<const vf4*>(qp + c)
-                            : vf4{qp[c * p.q.sd], qp[(c + 1) * p.q.sd], qp[(c + 2) * p.q.sd], qp[(c + 3) * p.q.sd]};
-            return x * p.qscale;
-        };
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if constexpr (BF16) {
-                const vf4 x = dims4(32 * s + 8 * g), y = dims4(32 * s + 8 * g + 4);
-                uint32_t w[3][4];
-                split3(x[0], x[1], w[0][0], w[1][0], w[2][0]);
-                split3(x[2], x[3], w[0][1], w[1][1], w[2][1]);
-                split3(y[0], y[1], w[0][2], w[1][2], w[2][2]);
-                split3(y[2], y[3], w[0][3], w[1][3], w[2][3]);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) qb[rt][s][i] = uintx4{w[i][0], w[i][1], w[i][2], w[i][3]};
-            } else {
-                qf[rt][s] = dims4(16 * s + 4 * g);
+            if (rok && (FULL || c < pool.d)) {
+                if (p.vec_q) {
+                    x = *reinterpret_cast<const vf4*>(qp + c);
+                } else {
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) x = vf4{x[1], x[2], x[3], qp[(c + k) * p.q.sd]};
+                }
             }
+            qx[i][y] = x;
         }
     }
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const int e = tid + 256 * i;
+        if (NRT * KS * 64 % 256 != 0 && e >= NRT * KS * 64) break;
+        uintx4* const to = smem + (e >> 6) * S::QP * 64 + (e & 63);
+        if constexpr (BF16) {
+            const vf4 x = qx[i][0] * p.qscale, y = qx[i][1] * p.qscale;
+            uint32_t w[3][4];
+            split3(x[0], x[1], w[0][0], w[1][0], w[2][0]);
+            split3(x[2], x[3], w[0][1], w[1][1], w[2][1]);
+            split3(y[0], y[1], w[0][2], w[1][2], w[2][2]);
+            split3(y[2], y[3], w[0][3], w[1][3], w[2][3]);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) to[64 * k] = uintx4{w[k][0], w[k][1], w[k][2], w[k][3]};
+        } else {
+            *to = __builtin_bit_cast(uintx4, qx[i][0] * p.qscale);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kTable / 256; ++i) table_s[tid + 256 * i] = page[i];
+
+    const int len = paged_clamp(pool, raw_len);
+    if (quotient(row0, p.by_g) >= count) return;                 // no token of this block exists
+    // Keys that some row sees, cut into equal parts of whole rounds of the waves.
+    const int seen = p.parents ? count : min(count, quotient(row0 + n_rows - 1, p.by_g) + 1);
+    const int n_keys = len + seen;
+    const int share = __builtin_amdgcn_readfirstlane((int)((float)n_keys * __builtin_amdgcn_rcpf((float)n_parts) * 1.000002f));
+    int part_len = (share + 4 * KB - 1) & ~(4 * KB - 1);
+    if (part_len * (int64_t)n_parts < n_keys) part_len += 4 * KB;
+    const int k0 = part * part_len, k1 = min(n_keys, k0 + part_len);
+    if (k0 >= k1) return;                            // part 0 always has keys
+    // Parts with keys: at most n_parts < 2^16, so the quotient in floats is off by one at most.
+    int live = __builtin_amdgcn_readfirstlane((int)((float)n_keys * __builtin_amdgcn_rcpf((float)part_len)));
+    live += live * (int64_t)part_len < n_keys;
+    live -= (live - 1) * (int64_t)part_len >= n_keys;
+    int tok[NRT];                        // token of row col of tile rt
+#pragma unroll
+    for (int rt = 0; rt < NRT; ++rt) tok[rt] = quotient(min(row0 + 16 * rt + col, p.R - 1), p.by_g);
 
     if (tid == 0) odd_s = 0;             // (the stage's barriers follow)
 
@@ -233,16 +286,15 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
     const int64_t row_bytes = (int64_t)pool.d * S::ES;
     typedef typename std::conditional<BF16 && VE == 4, uintx2, uintx4>::type VReg;
 
-    const int32_t* const table = pool.table + (int64_t)b * pool.max_pages;
     for (int kc = k0; kc < k1; kc += kStage) {
         const int n_stage = min(kStage, k1 - kc);
         const int n_blocks = (n_stage + KB - 1) / KB;
-        if (kc > k0) __syncthreads();
+        __syncthreads();                 // table_s is there; rows_s is done with
         bool bad = false;
         for (int i = tid; i < n_blocks * KB; i += 256) {
             int row = -1;
             if (i < n_stage) {
-                row = paged_row(pool, table, h, kc + i);
+                row = table_fits ? paged_row(pool, table_s, h, kc + i) : paged_row(pool, table, h, kc + i);
                 bad |= row < 0;
             }
             rows_s[i] = row;
@@ -257,7 +309,7 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
                 const char* row = kbase + max(rows_s[blk * KB + 16 * kt + col], 0) * row_bytes;
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
-                    kreg[kt][s] = load_vec<NT, uintx4>(row + S::ES * clamp_dim(BF16 ? 32 * s + 8 * g : 16 * s + 4 * g));
+                    kreg[kt][s] = load_vec<false, uintx4>(row + S::ES * clamp_dim(BF16 ? 32 * s + 8 * g : 16 * s + 4 * g));
             }
         };
         auto load_v = [&](int blk) __attribute__((always_inline)) {
@@ -281,7 +333,10 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
         }
         for (; blk < n_blocks; blk += 4) {
             const int kb = kc + blk * KB;
-            // ---- S^T = K Q^T
+            // ---- S^T = K Q^T (Q is read again for each block: held in registers
+            // it would cost a wave per SIMD, so its address is kept from being hoisted)
+            int qlane = lane;
+            asm volatile("" : "+v"(qlane));
             floatx4 s[NRT][KT];
 #pragma unroll
             for (int rt = 0; rt < NRT; ++rt)
@@ -290,19 +345,23 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
 #pragma unroll
             for (int st = 0; st < KS; ++st)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int rt = 0; rt < NRT; ++rt) {
+                    const uintx4* const qa = smem + (rt * KS + st) * S::QP * 64 + qlane;
+                    if constexpr (BF16) {
+                        const uintx4 q2 = qa[128], q1 = qa[64], q0 = qa[0];
 #pragma unroll
-                    for (int rt = 0; rt < NRT; ++rt) {
-                        if constexpr (BF16) {
+                        for (int kt = 0; kt < KT; ++kt) s[rt][kt] = mfma_part(kreg[kt][st], q2, s[rt][kt]);
 #pragma unroll
-                            for (int i = 2; i >= 0; --i) s[rt][kt] = mfma_part(kreg[kt][st], qb[rt][st][i], s[rt][kt]);
-                        } else {
-                            const vf4 kv = __builtin_bit_cast(vf4, kreg[kt][st]);
+                        for (int kt = 0; kt < KT; ++kt) s[rt][kt] = mfma_part(kreg[kt][st], q1, s[rt][kt]);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qf[rt][st][i], s[rt][kt], 0, 0, 0);
-                        }
+                        for (int kt = 0; kt < KT; ++kt) s[rt][kt] = mfma_part(kreg[kt][st], q0, s[rt][kt]);
+                    } else {
+                        const vf4 kv = __builtin_bit_cast(vf4, kreg[0][st]), qv = __builtin_bit_cast(vf4, *qa);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qv[i], s[rt][0], 0, 0, 0);
                     }
+                }
             const bool more = blk + 4 < n_blocks;
             if (more) load_k(blk + 4);
 
@@ -340,7 +399,7 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
             if (__builtin_amdgcn_ballot_w64(grow) != 0) {
 #pragma unroll
                 for (int rt = 0; rt < NRT; ++rt) {
-                    const float m_new = fmaxf(m_run[rt], m_blk[rt]);
+                    const float m_new = m_blk[rt] > m_run[rt] ? m_blk[rt] + kSlack : m_run[rt];
                     const float alpha = fast_exp2(m_run[rt] - (m_new == kNegInf ? 0.f : m_new));
                     m_run[rt] = m_new;
                     l_run[rt] *= alpha;
@@ -382,25 +441,34 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
 
             // ---- O^T += V^T P^T
             if constexpr (BF16) {
-                uintx4 vt[NO];               // dim c % VE of each load, two keys a register
+                uintx4 pb[NRT][3];
 #pragma unroll
-                for (int c = 0; c < NO; ++c)
+                for (int rt = 0; rt < NRT; ++rt)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        vt[c][k] = __builtin_amdgcn_perm(vreg[2 * k + 1][c / VE][(c % VE) / 2], vreg[2 * k][c / VE][(c % VE) / 2],
-                                                         c % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                for (int rt = 0; rt < NRT; ++rt) {
-                    uint32_t w[3][4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        split3(s[rt][k >> 1][2 * (k & 1)], s[rt][k >> 1][2 * (k & 1) + 1], w[0][k], w[1][k], w[2][k]);
-#pragma unroll
-                    for (int i = 2; i >= 0; --i) {
-                        const uintx4 pb = uintx4{w[i][0], w[i][1], w[i][2], w[i][3]};
-#pragma unroll
-                        for (int c = 0; c < NO; ++c) o[rt][c] = mfma_part(vt[c], pb, o[rt][c]);
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t w0, w1, w2;
+                        split3(s[rt][k >> 1][2 * (k & 1)], s[rt][k >> 1][2 * (k & 1) + 1], w0, w1, w2);
+                        pb[rt][0][k] = w0;
+                        pb[rt][1][k] = w1;
+                        pb[rt][2][k] = w2;
                     }
+                // Dims 2 c and 2 c + 1 of each load, two keys a register.
+#pragma unroll
+                for (int c = 0; c < NO; c += 2) {
+                    uintx4 even, odd;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = vreg[2 * k][c / VE][(c % VE) / 2], y = vreg[2 * k + 1][c / VE][(c % VE) / 2];
+                        even[k] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+                        odd[k] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                    }
+#pragma unroll
+                    for (int i = 2; i >= 0; --i)
+#pragma unroll
+                        for (int rt = 0; rt < NRT; ++rt) {
+                            o[rt][c] = mfma_part(even, pb[rt][i], o[rt][c]);
+                            o[rt][c + 1] = mfma_part(odd, pb[rt][i], o[rt][c + 1]);
+                        }
                 }
             } else {
 #pragma unroll
@@ -417,17 +485,37 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
         }
     }
 
+    // Writes dims dd..dd+3 of row rr: O over the sum of weights, zeros where nothing
+    // was seen.
+    auto put = [&](int rr, int dd, vf4 x, float l) __attribute__((always_inline)) {
+        const int r = row0 + rr, t = quotient(r, p.by_g);
+        if (t >= count) return;
+        float* const out = p.o.p + b * p.o.sb + (h * p.G + r - t * p.G) * p.o.sh + t * p.o.st;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        x = l == 0.f ? vf4{0.f, 0.f, 0.f, 0.f} : x * inv;
+        if (p.vec_o) {
+            if (FULL || dd < pool.d) *reinterpret_cast<vf4*>(out + dd) = x;
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                if (dd + i < pool.d) out[(dd + i) * p.o.sd] = x[0];
+                x = vf4{x[1], x[2], x[3], x[0]};
+            }
+        }
+    };
+
     // ---- the 4 waves' (m, l, O), one tile of rows at a time
     const int64_t rec_floats = paged_record_floats(p.rec_rows, D);
     const int o_at = (2 * p.rec_rows + 3) & ~3;          // O of a record
     const int heads_blocks = pool.Hkv * p.n_rb;
     const int64_t rec0 = ((int64_t)p.prefix[bl] * pool.Hkv + h) * p.n_rb + rb;   // part 0's record
-    float* const rec = p.ws + (rec0 + (int64_t)part * heads_blocks) * rec_floats;
+    const __amdgpu_buffer_rsrc_t rec_range = coherent_range(p.ws + (rec0 + (int64_t)part * heads_blocks) * rec_floats,
+                                                            live > 1 ? (uint32_t)rec_floats * 4u : 0u);
 #pragma unroll
     for (int rt = 0; rt < NRT; ++rt) {
         if (16 * rt >= n_rows) break;
         const float l_all = row_groups_sum(l_run[rt]);
-        if (rt > 0) __syncthreads();
+        __syncthreads();                 // Q, or the tile before, is done with
 #pragma unroll
         for (int c = 0; c < NO; c += 4)
 #pragma unroll
@@ -455,7 +543,7 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
                 acc += f * *reinterpret_cast<const vf4*>(ob + (w * 16 + lr) * OS + dd);
             }
             if (odd_s) {                 // values that are not finite, for the rows that see them
-                const int t = (row0 + rr) / p.G;
+                const int t = quotient(row0 + rr, p.by_g);
                 for (int key = max(k0, len); key < k1; ++key) {
                     const int row = paged_row(pool, table, h, key);
                     if (row < 0 || !sees(t, key - len)) continue;
@@ -469,19 +557,10 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
                 }
             }
             if (live == 1) {
-                const int r = row0 + rr, t = r / p.G;
-                if (t >= count) continue;
-                float* out = p.o.p + b * p.o.sb + (h * p.G + r % p.G) * p.o.sh + t * p.o.st;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (FULL || dd + i < pool.d) out[(dd + i) * p.o.sd] = l == 0.f ? 0.f : acc[i] / l;
+                put(rr, dd, acc, l);
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) store_coherent(rec + o_at + rr * D + dd + i, acc[i]);
-                if (dd == 0) {
-                    store_coherent(rec + 2 * rr, M);
-                    store_coherent(rec + 2 * rr + 1, l);
-                }
+                store_coherent4(rec_range, (uint32_t)(4 * (o_at + rr * D + dd)), acc);
+                if (dd == 0) store_coherent2(rec_range, (uint32_t)(8 * rr), M, l);
             }
         }
     }
@@ -496,45 +575,60 @@ __global__ __launch_bounds__(256, NRT == 1 && D <= 128 ? 2 : 1) void paged_atten
     __syncthreads();
     if (!last_s) return;
     if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int64_t step = heads_blocks * rec_floats;       // floats between two parts' records
-    const float* const first = p.ws + rec0 * rec_floats;
-    constexpr int NR = 8;                                 // records a thread has in flight
-    for (int e = tid; e < n_rows * (D / 4); e += 256) {
-        const int rr = e / (D / 4), dd = 4 * (e % (D / 4));
-        float M = kNegInf, l = 0.f;
-        vf4 acc = vf4{0.f, 0.f, 0.f, 0.f};
+    // Each thread combines EV groups of 4 dims, with the loads of NR records of
+    // all of them in flight (a trip to the coherence point is about 1.2 us: with 8
+    // loads a trip the merge of 14 records of 32 rows took 13 us of a 26 us launch).
+    constexpr int VPT = (ROWS * D / 4 + 255) / 256, EV = VPT < 4 ? VPT : 4, NR = (NRT == 1 ? 16 : 32) / EV;
+    const uint32_t step = (uint32_t)(heads_blocks * rec_floats * 4);     // bytes between two parts' records
+    const __amdgpu_buffer_rsrc_t range = coherent_range(p.ws + rec0 * rec_floats,
+                                                        (uint32_t)(live - 1) * step + (uint32_t)rec_floats * 4u);
+    for (int e0 = tid; e0 < n_rows * (D / 4); e0 += 256 * EV) {
+        float M[EV], l[EV];
+        vf4 acc[EV];
+#pragma unroll
+        for (int v = 0; v < EV; ++v) {
+            M[v] = kNegInf;
+            l[v] = 0.f;
+            acc[v] = vf4{0.f, 0.f, 0.f, 0.f};
+        }
         for (int c0 = 0; c0 < live; c0 += NR) {
-            float2 ml[NR];
-            vf4 x[NR];
-#pragma unroll
-            for (int c = 0; c < NR; ++c) {
-                const float* at = first + min(c0 + c, live - 1) * step;
-                const __amdgpu_buffer_rsrc_t range = coherent_range(at, (uint32_t)rec_floats * 4u);
-                ml[c] = load_coherent2(range, (uint32_t)(8 * rr));
-                x[c] = load_coherent4(range, (uint32_t)(4 * (o_at + rr * D + dd)));
-            }
-            float M_new = M;
-#pragma unroll
-            for (int c = 0; c < NR; ++c) M_new = fmaxf(M_new, ml[c].x);
-            const float M_use = M_new == kNegInf ? 0.f : M_new;
-            const float old = fast_exp2(M - M_use);
-            l *= old;
-            acc *= old;
-            M = M_new;
+            float2 ml[EV][NR];
+            vf4 x[EV][NR];
 #pragma unroll
             for (int c = 0; c < NR; ++c)
-                if (c0 + c < live) {
-                    const float f = fast_exp2(ml[c].x - M_use);
-                    l += f * ml[c].y;
-                    acc += f * x[c];
-                }
-        }
-        const int r = row0 + rr, t = r / p.G;
-        if (t >= count) continue;
-        float* out = p.o.p + b * p.o.sb + (h * p.G + r % p.G) * p.o.sh + t * p.o.st;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (FULL || dd + i < pool.d) out[(dd + i) * p.o.sd] = l == 0.f ? 0.f : acc[i] / l;
+                for (int v = 0; v < EV; ++v) {       // (past the last record: zeros, without an access)
+                    const int e = e0 + 256 * v, rr = e / (D / 4), dd = 4 * (e % (D / 4));
+                    const uint32_t at = e < n_rows * (D / 4) ? (uint32_t)(c0 + c) * step : 0xfffffff0u - 4u * ROWS * (D + 2);
+                    ml[v][c] = load_coherent2(range, at + 8u * rr);
+                    x[v][c] = load_coherent4(range, at + 4u * (o_at + rr * D + dd));
+                }
+#pragma unroll
+            for (int v = 0; v < EV; ++v) {
+                float M_new = M[v];
+#pragma unroll
+                for (int c = 0; c < NR; ++c) {
+                    ml[v][c].x = c0 + c < live ? ml[v][c].x : kNegInf;
+                    M_new = fmaxf(M_new, ml[v][c].x);
+                }
+                const float M_use = M_new == kNegInf ? 0.f : M_new;
+                const float old = fast_exp2(M[v] - M_use);
+                l[v] *= old;
+                acc[v] *= old;
+                M[v] = M_new;
+#pragma unroll
+                for (int c = 0; c < NR; ++c) {
+                    const float f = fast_exp2(ml[v][c].x - M_use);
+                    l[v] += f * ml[v][c].y;
+                    acc[v] += f * x[v][c];
+                }
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < EV; ++v) {
+            const int e = e0 + 256 * v, rr = e / (D / 4), dd = 4 * (e % (D / 4));
+            if (rr < n_rows) put(rr, dd, acc[v], l[v]);
+        }
     }
 }
 
@@ -550,21 +644,20 @@ hipError_t launch_tile(const PagedAttnParams& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <bool BF16, int D>
+hipError_t launch_dim(const PagedAttnParams& p, hipStream_t stream) {
+    // (one row block: each byte of K and V is read by one workgroup)
+    if (p.tile_rows == 16)
+        return p.n_rb == 1 ? launch_tile<BF16, D, 1, true>(p, stream) : launch_tile<BF16, D, 1, false>(p, stream);
+    return launch_tile<BF16, D, 2, false>(p, stream);
+}
+
 template <bool BF16>
 hipError_t launch_type(const PagedAttnParams& p, hipStream_t stream) {
-    const int rows = paged_tile_rows(p.R, p.pool.d);
     switch (paged_tile_dim(p.pool.d)) {
-    case 64:
-        return rows == 16 ? launch_tile<BF16, 64, 1, true>(p, stream)
-             : rows == 32 ? launch_tile<BF16, 64, 2, true>(p, stream)
-                          : launch_tile<BF16, 64, 4, false>(p, stream);
-    case 128:
-        return rows == 16 ? launch_tile<BF16, 128, 1, true>(p, stream)
-             : rows == 32 ? launch_tile<BF16, 128, 2, true>(p, stream)
-                          : launch_tile<BF16, 128, 4, false>(p, stream);
-    default:
-        return rows == 16 ? launch_tile<BF16, 256, 1, true>(p, stream)
-                          : launch_tile<BF16, 256, 2, false>(p, stream);
+    case 64: return launch_dim<BF16, 64>(p, stream);
+    case 128: return launch_dim<BF16, 128>(p, stream);
+    default: return launch_dim<BF16, 256>(p, stream);
     }
 }
 

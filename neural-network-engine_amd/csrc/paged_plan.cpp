@@ -10,8 +10,9 @@ namespace {
 constexpr int kTargetPerCu = 4;    // workgroups per CU that a split may make
 }
 
-int64_t paged_max_records(int64_t B, int64_t heads_blocks, int cus) {
-    return (int64_t)kTargetPerCu * cus + B * heads_blocks;
+int64_t paged_max_records(int64_t B, int64_t units, int64_t record_bytes, int cus) {
+    const int64_t n = (int64_t)kTargetPerCu * cus + B * units;
+    return n * record_bytes <= kPagedRecordBytes ? n : 0;
 }
 
 int paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
@@ -24,15 +25,17 @@ int paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
     // Part lengths from the longest sequence down to 64 keys; the one of least
     // modelled time: a workgroup pays a fixed time and its keys, as many run at
     // once as the device holds, and a sequence in parts pays their merge.
+    const int64_t step = p.pool.bf16 ? 128 : 64;           // keys of a round of the waves
     const int64_t slots = 2 * (int64_t)cus;
+    const int64_t most = paged_max_records(p.B, units, 4 * paged_record_floats(p.rec_rows, paged_tile_dim(p.pool.d)), cus);
     int64_t best_len = longest;
     double best = 1e300;
     for (int64_t n = 1; n <= 512; n = n < 8 ? n + 1 : n + n / 4) {
-        const int64_t len = std::max<int64_t>(64, ((longest + n - 1) / n + 31) / 32 * 32);
+        const int64_t len = ((longest + n - 1) / n + step - 1) / step * step;
         int64_t parts = 0;
         for (int b = 0; b < p.B; ++b) parts += std::max<int64_t>(1, (keys[b] + len - 1) / len);
         const int64_t wgs = parts * units;
-        if (n > 1 && wgs > (int64_t)kTargetPerCu * cus + p.B * units) break;
+        if (n > 1 && wgs > most) break;
         const int64_t rounds = (wgs + slots - 1) / slots;
         // Long launches flow through the device, short ones run in rounds.
         const double flow = (double)total * units / slots;
@@ -40,11 +43,11 @@ int paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
                                                  : flow + 150.0 * rounds + 0.5 * (double)len)
                             + (n > 1 ? 100.0 + 12.0 * (double)n : 0.0);
         if (time < best) { best = time; best_len = len; }
-        if (len == 64) break;
+        if (len == step) break;
     }
     p.prefix[0] = 0;
     for (int b = 0; b < p.B; ++b)
-        p.prefix[b + 1] = p.prefix[b] + (int)std::max<int64_t>(1, (keys[b] + best_len - 1) / best_len);
+        p.prefix[b + 1] = (uint16_t)(p.prefix[b] + std::max<int64_t>(1, (keys[b] + best_len - 1) / best_len));
     return p.prefix[p.B];
 }
 
