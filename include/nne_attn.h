@@ -380,7 +380,8 @@ enum { NNE_F32 = 0, NNE_BF16 = 1 };
 typedef struct nne_paged_cache {
     void *k, *v;               /* one layer's pools, 16-byte aligned */
     int64_t dtype;             /* NNE_F32 or NNE_BF16 */
-    int64_t n_pages, Hkv, page_size, d;   /* n_pages * Hkv * page_size < 2^31 */
+    int64_t n_pages, Hkv, page_size, d;   /* n_pages * Hkv * page_size < 2^31 rows
+                                             and 64 GiB */
     int64_t B, max_pages;      /* sequences, pages a sequence may have */
     const int32_t *table;      /* device [B][max_pages] */
     const int32_t *table_host; /* host copy, or NULL */

@@ -914,29 +914,28 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6
     rope=None: no rotation; eps=None: no norm, the rotation alone (no weights);
     k=None: q alone.  Returns (q_out, k_out): new tensors in the inputs' order of dims
     by default, or the given ones (q and k themselves are fine)."""
-    qs, qst = _shape4(q, "Q")
-    index = q.get_device()
-    _check_f32(index, q)
+    qs, index = q.shape, q.get_device()
+    _check_f32(index, *[t for t in (q, k, q_weight, k_weight) if t is not None])
+    if len(qs) != 4 or (k is not None and k.dim() != 4):
+        _shape4(q, "Q")
+        _shape4(k, "K")
     b, _, t, d = qs
     for w in (q_weight, k_weight):
-        if w is not None:
-            _check_f32(index, w)
-            if w.shape != (d,) or not w.is_contiguous():
-                raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
-                                    % ([d], list(w.shape)))
+        if w is not None and (w.dim() != 1 or w.numel() != d or not w.is_contiguous()):
+            raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
+                                % ([d], list(w.shape)))
     if q_out is None:
         q_out = _new_like(q, stream)
     else:
         _check_out(q_out, qs, index)
     ks = _NO_K
     if k is not None:
-        _check_f32(index, k)
-        kshape, kst = _shape4(k, "K")
+        kshape = k.shape
         if k_out is None:
             k_out = _new_like(k, stream)
         else:
             _check_out(k_out, kshape, index)
-        ks = (k.data_ptr(), kshape, kst, k_out.data_ptr(), k_out.stride())
+        ks = (k.data_ptr(), kshape, k.stride(), k_out.data_ptr(), k_out.stride())
     elif k_out is not None:
         raise InvalidArgument("Invalid configuration or argument: k_out without k")
     start, depths = _NO_PAIR, _NO_PAIR
@@ -947,12 +946,14 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6
         if draft is not None:
             draft._check(b, t, index)
             depths = draft._depths
-    check(_native().qk_norm_rope(
-        q.data_ptr(), qs, qst, q_out.data_ptr(), q_out.stride(), *ks,
+    rc = _native().qk_norm_rope(
+        q.data_ptr(), qs, q.stride(), q_out.data_ptr(), q_out.stride(), *ks,
         None if q_weight is None else q_weight.data_ptr(),
         None if k_weight is None else k_weight.data_ptr(), eps is not None,
         0.0 if eps is None else eps, *_rope_args(rope, index), *start, *depths,
-        _stream_on(index, stream)))
+        _stream_on(index, stream))
+    if rc:
+        check(rc)
     return q_out, k_out
 
 
@@ -1176,7 +1177,9 @@ class PagedKVCache:
         self._check_layer(layer_idx)
         index = self._index
         _check_f32(index, k_new, v_new)
-        shape, kst = _shape4(k_new, "K")
+        shape = k_new.shape
+        if len(shape) != 4:
+            _shape4(k_new, "K")
         b, h, t, d = shape
         if b != self.batch or h != self.num_kv_heads or d != self.head_dim or v_new.shape != shape:
             raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s" % (
@@ -1186,9 +1189,12 @@ class PagedKVCache:
         if draft is not None:
             draft._check(b, t, index)
             counts, depths = draft._counts, draft._depths
-        check(_native().paged_append(
-            self._addr[layer_idx][0], k_new.data_ptr(), kst, v_new.data_ptr(), v_new.stride(), t,
-            *counts, *depths, *_rope_args(rope, index), _stream_on(index, stream)))
+        rc = _native().paged_append(
+            self._addr[layer_idx][0], k_new.data_ptr(), k_new.stride(), v_new.data_ptr(),
+            v_new.stride(), t, *counts, *depths, *_rope_args(rope, index),
+            _stream_on(index, stream))
+        if rc:
+            check(rc)
 
     def attend(self, layer_idx, q, draft=None, out=None, scale=None, stream=None):
         """Attention of the appended tokens' queries q [B, Hq, T, d] over the
@@ -1198,7 +1204,9 @@ class PagedKVCache:
         self._check_layer(layer_idx)
         index = self._index
         _check_f32(index, q)
-        shape, qst = _shape4(q, "Q")
+        shape = q.shape
+        if len(shape) != 4:
+            _shape4(q, "Q")
         b, hq, t, d = shape
         if b != self.batch or d != self.head_dim or hq == 0 or hq % self.num_kv_heads != 0:
             raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s" % (
@@ -1213,10 +1221,12 @@ class PagedKVCache:
             counts, parents = draft._counts, draft._parents
         if t == 0:
             return out
-        check(_native().paged_attention(
-            self._addr[layer_idx][1], q.data_ptr(), qst, out.data_ptr(), out.stride(), hq, t,
-            *counts, *parents, scale is not None, 0.0 if scale is None else scale,
-            self._ws_args(hq, t, stream), _stream_on(index, stream)))
+        rc = _native().paged_attention(
+            self._addr[layer_idx][1], q.data_ptr(), q.stride(), out.data_ptr(), out.stride(), hq,
+            t, *counts, *parents, scale is not None, 0.0 if scale is None else scale,
+            self._ws_args(hq, t, stream), _stream_on(index, stream))
+        if rc:
+            check(rc)
         return out
 
     def commit(self, counts, counts_host=None, paths=None, paths_host=None, stream=None):

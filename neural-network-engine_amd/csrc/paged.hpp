@@ -57,7 +57,8 @@ struct PagedAttnParams {
     int B;                     // sequences of the launch
     float* ws;                 // records: (max, sum) and O of rec_rows rows each
     uint32_t* cnt;             // arrivals per (sequence, KV head, row block)
-    // Sequence b's keys are cut into parts prefix[b + 1] - prefix[b], numbered
+    int combine;               // records are merged by a kernel of their own, not by the last to arrive
+    // Sequence b's keys are cut into prefix[b + 1] - prefix[b] equal parts, numbered
     // through the launch.
     uint16_t prefix[kPagedSeqs + 1];
 };
@@ -78,9 +79,9 @@ inline int64_t paged_record_floats(int rows, int D) { return ((2 * rows + 3) & ~
 constexpr int64_t kPagedRecordBytes = int64_t{1} << 28;
 int64_t paged_max_records(int64_t B, int64_t units, int64_t record_bytes, int cus);
 
-// Fills p.prefix for sequences of keys[b] keys (p's sizes set); returns the number
-// of parts.
-int paged_plan(PagedAttnParams& p, const int64_t* keys, int cus);
+// Fills p.prefix and p.combine for sequences of keys[b] keys (p's sizes set);
+// returns the number of records (0: nothing is split).
+int64_t paged_plan(PagedAttnParams& p, const int64_t* keys, int cus);
 
 struct PagedAppendParams {
     View4 k, v;

@@ -50,6 +50,10 @@ int check_cache(const nne_paged_cache_t* c, int64_t T) {
     if (c->d <= 0 || c->d % 8 != 0 || c->d > nne::kPagedMaxDim)
         return fail_format(NNE_EINVAL, NNE_BAD "paged cache head dim %lld must be a multiple of 8 up to %d",
                            (long long)c->d, nne::kPagedMaxDim);
+    const int64_t bytes = c->n_pages * c->Hkv * c->page_size * c->d * (c->dtype == NNE_BF16 ? 2 : 4);
+    if (bytes >= int64_t{1} << 36)
+        return fail_format(NNE_EINVAL, NNE_BAD "a layer's pool of %lld bytes: K and V may have 64 GiB each",
+                           (long long)bytes);
     if (T < 0 || T > INT32_MAX || c->max_pages * c->page_size + T > INT32_MAX)
         return fail_format(NNE_EINVAL, NNE_BAD "%lld tokens behind %lld pages of %lld rows", (long long)T,
                            (long long)c->max_pages, (long long)c->page_size);
@@ -388,14 +392,15 @@ int nne_paged_attention(const nne_paged_cache_t* cache, const float* q, const in
             const int64_t n = count_of(counts_host, b0 + i, T);
             keys[i] = n > 0 ? cache->lens_host[b0 + i] + n : 1;
         }
-        const int64_t parts = nne::paged_plan(p, keys, nne::cus_of_device());
+        const int64_t n_records = nne::paged_plan(p, keys, nne::cus_of_device());
         p.ws = nullptr;
         p.cnt = nullptr;
-        if (parts > p.B) {
-            const int64_t units = (int64_t)p.pool.Hkv * p.n_rb;
+        if (n_records > 0) {
             void* records = nullptr;
-            rc = nne::take_workspace(ws, (uint64_t)(parts * units * rec_bytes), p.B * units, s, &records, &p.cnt,
+            rc = nne::take_workspace(ws, (uint64_t)(n_records * rec_bytes),
+                                     p.combine ? 0 : (int64_t)p.B * p.pool.Hkv * p.n_rb, s, &records, &p.cnt,
                                      "paged attention");
+            if (p.combine) p.cnt = nullptr;
             if (rc) return rc;
             p.ws = static_cast<float*>(records);
         }

@@ -36,7 +36,6 @@ namespace nne {
 namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
@@ -98,14 +97,66 @@ __device__ __forceinline__ int slot_key(int g, int j) {
     return BF16 ? 16 * (j >> 2) + 4 * g + (j & 3) : 4 * g + j;
 }
 
+// n / d for uniform n >= 0, d > 0 with a quotient below 2^16 (off by one at most
+// before it is put right).
+__device__ __forceinline__ int small_quotient(int n, int d) {
+    int q = __builtin_amdgcn_readfirstlane((int)((float)n * __builtin_amdgcn_rcpf((float)d)));
+    q -= q * (int64_t)d > n;
+    q += (q + 1) * (int64_t)d <= n;
+    return q;
+}
+
 __device__ __forceinline__ bool not_finite(float x) {
     return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 }
 
+// Writes dims dd..dd+3 of row r of a KV head: O over the sum of weights, zeros
+// where nothing was seen.
+__device__ __forceinline__ void put_row4(const PagedAttnParams& p, int b, int h, int r, int count, int dd, vf4 x, float l) {
+    const int t = quotient(r, p.by_g);
+    if (t >= count) return;
+    float* const out = p.o.p + b * p.o.sb + (h * p.G + r - t * p.G) * p.o.sh + t * p.o.st;
+    x = l == 0.f ? vf4{0.f, 0.f, 0.f, 0.f} : x * (1.f / l);
+    if (p.vec_o) {
+        if (dd < p.pool.d) *reinterpret_cast<vf4*>(out + dd) = x;
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+            if (dd + i < p.pool.d) out[(dd + i) * p.o.sd] = x[0];
+            x = vf4{x[1], x[2], x[3], x[0]};
+        }
+    }
+}
+
+// Keys that some row of the block sees (0: none of its tokens exists).
+__device__ __forceinline__ int block_keys(const PagedAttnParams& p, int row0, int n_rows, int len, int count) {
+    if (quotient(row0, p.by_g) >= count) return 0;
+    return len + (p.parents ? count : min(count, quotient(row0 + n_rows - 1, p.by_g) + 1));
+}
+
+// How many parts a (sequence, KV head, row block)'s keys are in, of how many keys
+// (whole rounds of the waves), and where their records lie.  n: its parts as planned.
+struct Parts {
+    int live, length;
+    int64_t rec0, rec_step;
+};
+
+__device__ __forceinline__ Parts even_parts(const PagedAttnParams& p, int before, int n, int h, int rb, int n_keys, int round) {
+    Parts r;
+    const int even = __builtin_amdgcn_readfirstlane((int)((float)n_keys * __builtin_amdgcn_rcpf((float)n) * 1.000002f));
+    r.length = (even + round - 1) & ~(round - 1);
+    if (r.length * (int64_t)n < n_keys) r.length += round;
+    r.live = n_keys > 0 ? small_quotient(n_keys + r.length - 1, r.length) : 0;
+    r.rec_step = p.pool.Hkv * p.n_rb;
+    r.rec0 = ((int64_t)before * p.pool.Hkv + h) * p.n_rb + rb;
+    return r;
+}
+
 // BF16: the pools' type.  D: dims, padded.  NRT: 16-row tiles of query rows.
-// FULL: d == D.  NT: no other workgroup reads these keys.
-template <bool BF16, int D, int NRT, bool FULL, bool NT>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(const PagedAttnParams p) {
+// FULL: d == D.  NT: no other workgroup reads these keys.  DRAFT: T > 1, rows may see
+// different keys (its masks cost a third wave per SIMD in registers).
+template <bool BF16, int D, int NRT, bool FULL, bool NT, bool DRAFT>
+__global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attention_kernel(const PagedAttnParams p) {
     using S = Shape<BF16, D>;
     constexpr int KB = S::KB, JN = S::JN, VE = S::VE, NV = S::NV, KT = S::KT, KS = S::KS, NO = S::NO;
     constexpr int OS = D + 4;                        // row stride of the merge buffer
@@ -117,26 +168,26 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
     constexpr int ON = 4 * 16 * OS / 4;
     __shared__ uintx4 smem[QN > ON ? QN : ON];
     float* const ob = reinterpret_cast<float*>(smem);
-    __shared__ __attribute__((aligned(16))) int rows_s[kStage];
+    __shared__ __attribute__((aligned(16))) uint32_t rows_s[kStage];   // 16-byte units from the pool
+    __shared__ uint32_t gone_s[kStage / 32];     // keys without a row, a bit each
     __shared__ float ml_s[4][16][2];
     __shared__ uint32_t anc_s[kPagedTreeNodes][kPagedTreeNodes / 32];
     __shared__ int nxt_s[kPagedTreeNodes];
     __shared__ int table_s[kTable];
     __shared__ int last_s, odd_s;
 
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int col = lane & 15, g = lane >> 4;
-    const PagedPool& pool = p.pool;
     // Everything up to the first K and V is latency: one trip for the arguments,
     // one for the length, the page table and Q together, one for K and V.
     const int pref_lo = p.prefix[min(lane + 1, kPagedSeqs)], pref_hi = p.prefix[min(lane + 65, kPagedSeqs)];
     warm_kernargs<0, sizeof(PagedAttnParams)>();
     asm volatile("" ::"v"(pref_lo), "v"(pref_hi));
+    const PagedPool& pool = p.pool;
 
-    // Workgroup -> (part and KV head, row block).  With several row blocks, the
-    // ones that read the same keys follow each other on one XCD (workgroups go to
-    // the 8 XCDs in turn), whose L2 then serves them.
+    // Workgroup -> (part of a sequence and KV head, row block).  With several row
+    // blocks, the ones that read the same keys follow each other on one XCD
+    // (workgroups go to the 8 XCDs in turn), whose L2 then serves them.
     int unit = blockIdx.x, rb = 0;
     if (p.n_rb > 1) {
         const int x = unit & 7, y = unit >> 3, z = quotient(y, p.by_rb);
@@ -145,15 +196,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
     }
     if (unit >= p.prefix[p.B] * pool.Hkv) return;
     const int part_all = quotient(unit, p.by_hkv), h = unit - part_all * pool.Hkv;
-    int bl;
-    {
-        const int lo = lane < p.B ? pref_lo : INT32_MAX, hi = lane + 64 < p.B ? pref_hi : INT32_MAX;
-        bl = __popcll(__builtin_amdgcn_ballot_w64(lo <= part_all)) +
-             __popcll(__builtin_amdgcn_ballot_w64(hi <= part_all));
-    }
-    const int part = part_all - p.prefix[bl], n_parts = p.prefix[bl + 1] - p.prefix[bl];
+    const int bl = __popcll(__builtin_amdgcn_ballot_w64(lane < p.B && pref_lo <= part_all)) +
+                   __popcll(__builtin_amdgcn_ballot_w64(lane + 64 < p.B && pref_hi <= part_all));
     const int b = p.b0 + bl;
-
     const int row0 = rb * ROWS;
     const int n_rows = min(ROWS, p.R - row0);
     const int raw_len = pool.lens[b];
@@ -211,20 +256,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
 #pragma unroll
     for (int i = 0; i < kTable / 256; ++i) table_s[tid + 256 * i] = page[i];
 
+    // This part's keys, k0 to k1 of those that some row sees.
     const int len = paged_clamp(pool, raw_len);
-    if (quotient(row0, p.by_g) >= count) return;                 // no token of this block exists
-    // Keys that some row sees, cut into equal parts of whole rounds of the waves.
-    const int seen = p.parents ? count : min(count, quotient(row0 + n_rows - 1, p.by_g) + 1);
-    const int n_keys = len + seen;
-    const int share = __builtin_amdgcn_readfirstlane((int)((float)n_keys * __builtin_amdgcn_rcpf((float)n_parts) * 1.000002f));
-    int part_len = (share + 4 * KB - 1) & ~(4 * KB - 1);
-    if (part_len * (int64_t)n_parts < n_keys) part_len += 4 * KB;
-    const int k0 = part * part_len, k1 = min(n_keys, k0 + part_len);
-    if (k0 >= k1) return;                            // part 0 always has keys
-    // Parts with keys: at most n_parts < 2^16, so the quotient in floats is off by one at most.
-    int live = __builtin_amdgcn_readfirstlane((int)((float)n_keys * __builtin_amdgcn_rcpf((float)part_len)));
-    live += live * (int64_t)part_len < n_keys;
-    live -= (live - 1) * (int64_t)part_len >= n_keys;
+    const int n_keys = block_keys(p, row0, n_rows, len, count);
+    const Parts parts = even_parts(p, p.prefix[bl], p.prefix[bl + 1] - p.prefix[bl], h, rb, n_keys, 4 * KB);
+    const int part = part_all - p.prefix[bl], live = parts.live;
+    const int k0 = min(part * (int64_t)parts.length, (int64_t)n_keys);
+    const int k1 = min((int64_t)n_keys, k0 + (int64_t)parts.length);
+    if (k0 >= k1) return;
     int tok[NRT];                        // token of row col of tile rt
 #pragma unroll
     for (int rt = 0; rt < NRT; ++rt) tok[rt] = quotient(min(row0 + 16 * rt + col, p.R - 1), p.by_g);
@@ -233,7 +272,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
 
     // Which drafted tokens precede a token: bit u of anc_s[t].  Pointer
     // doubling: after k rounds a row holds its 2^k nearest.
-    if (p.parents && k1 > len) {
+    if (DRAFT && p.parents && k1 > len) {
         constexpr int W = kPagedTreeNodes / 32;
         const int words = (p.T + 31) / 32;
         uint32_t own[W];
@@ -283,30 +322,31 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
     const auto clamp_dim = [&](int c) __attribute__((always_inline)) { return FULL || c < pool.d ? c : 0; };
     const char* const kbase = static_cast<const char*>(pool.k);
     const char* const vbase = static_cast<const char*>(pool.v);
-    const int64_t row_bytes = (int64_t)pool.d * S::ES;
+    const uint32_t row_units = (uint32_t)pool.d * S::ES / 16;      // (the host keeps pools below 2^32 units)
+    // A row's address: one shift-and-add where row numbers would take a 64-bit
+    // multiplication (16 cycles a wave) for each of a block's rows.
+    const auto row_at = [](const char* base, uint32_t at) __attribute__((always_inline)) { return base + ((uint64_t)at << 4); };
     typedef typename std::conditional<BF16 && VE == 4, uintx2, uintx4>::type VReg;
 
     for (int kc = k0; kc < k1; kc += kStage) {
         const int n_stage = min(kStage, k1 - kc);
         const int n_blocks = (n_stage + KB - 1) / KB;
         __syncthreads();                 // table_s is there; rows_s is done with
-        bool bad = false;
         for (int i = tid; i < n_blocks * KB; i += 256) {
             int row = -1;
-            if (i < n_stage) {
-                row = table_fits ? paged_row(pool, table_s, h, kc + i) : paged_row(pool, table, h, kc + i);
-                bad |= row < 0;
-            }
-            rows_s[i] = row;
+            if (i < n_stage) row = table_fits ? paged_row(pool, table_s, h, kc + i) : paged_row(pool, table, h, kc + i);
+            rows_s[i] = (uint32_t)max(row, 0) * row_units;           // (row 0 where there is none: not used)
+            const uint64_t gone = __builtin_amdgcn_ballot_w64(row < 0);
+            if ((lane & 31) == 0) gone_s[i >> 5] = (uint32_t)(gone >> (lane & 32));
         }
-        const bool holes = __syncthreads_or(bad) != 0;
+        __syncthreads();
 
         uintx4 kreg[KT][KS];
         VReg vreg[JN][NV];
         auto load_k = [&](int blk) __attribute__((always_inline)) {
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                const char* row = kbase + max(rows_s[blk * KB + 16 * kt + col], 0) * row_bytes;
+                const char* row = row_at(kbase, rows_s[blk * KB + 16 * kt + col]);
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
                     kreg[kt][s] = load_vec<false, uintx4>(row + S::ES * clamp_dim(BF16 ? 32 * s + 8 * g : 16 * s + 4 * g));
@@ -315,10 +355,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
         auto load_v = [&](int blk) __attribute__((always_inline)) {
 #pragma unroll
             for (int q = 0; q < JN / 4; ++q) {
-                const intx4 r4 = *reinterpret_cast<const intx4*>(rows_s + blk * KB + 16 * q + 4 * g);
+                const uintx4 r4 = *reinterpret_cast<const uintx4*>(rows_s + blk * KB + 16 * q + 4 * g);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const char* row = vbase + max(r4[i], 0) * row_bytes;
+                    const char* row = row_at(vbase, r4[i]);
 #pragma unroll
                     for (int c = 0; c < NV; ++c)
                         vreg[4 * q + i][c] = load_vec<NT, VReg>(row + S::ES * clamp_dim(16 * VE * c + VE * col));
@@ -366,12 +406,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
             if (more) load_k(blk + 4);
 
             // ---- masks: only the last blocks have any
-            const bool drafted = p.T > 1 && kb + KB > len;
-            if (holes || kb + KB > k1 || drafted) {
+            const bool drafted = DRAFT && p.T > 1 && kb + KB > len;
+            const uint32_t gone = (uint32_t)__builtin_amdgcn_readfirstlane((int)gone_s[blk * KB >> 5]) >> (blk * KB & 31);
+            if (__builtin_expect((gone << (32 - KB)) != 0 || drafted, 0)) {
+                int gm = g;              // (nothing of this is worth a register in the other blocks)
+                asm volatile("" : "+v"(gm));
 #pragma unroll
                 for (int j = 0; j < JN; ++j) {
-                    const int in = slot_key<BF16>(g, j);
-                    const bool there = rows_s[blk * KB + in] >= 0;
+                    const int in = slot_key<BF16>(gm, j);
+                    const bool there = ((gone >> in) & 1u) == 0;
 #pragma unroll
                     for (int rt = 0; rt < NRT; ++rt) {
                         const bool ok = there & (!drafted | sees(tok[rt], kb + in - len));
@@ -423,20 +466,24 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
             // ---- where rows see different keys: a V that is not finite would
             // reach the rows that do not see it as 0 * inf.  Such values are taken
             // out here and added to the rows that see them at the end.
-            if (drafted) {
-                bool odd = false;
+            if (__builtin_expect(drafted, 0)) {
+                uint32_t fine = ~0u;
 #pragma unroll
-                for (int j = 0; j < JN; ++j)
+                for (int j = 0; j < JN; ++j) {
 #pragma unroll
                     for (int c = 0; c < NV; ++c)
 #pragma unroll
                         for (int w = 0; w < (int)(sizeof(VReg) / 4); ++w) {
+                            // (all ones where the exponent is not: no comparison, whose
+                            // results would take scalar registers)
                             const uint32_t x = vreg[j][c][w];
-                            const bool lo = BF16 && (x & 0x7f80u) == 0x7f80u, hi = (x & 0x7f800000u) == 0x7f800000u;
-                            odd |= lo | hi;
-                            vreg[j][c][w] = x & (lo ? 0xffff0000u : ~0u) & (hi ? (BF16 ? 0x0000ffffu : 0u) : ~0u);
+                            const uint32_t hi = (uint32_t)((int)((x & 0x7f800000u) - 0x7f800000u) >> 31);
+                            const uint32_t lo = BF16 ? (uint32_t)((int)((x & 0x7f80u) - 0x7f80u) >> 31) : hi;
+                            fine &= hi & lo;
+                            vreg[j][c][w] = x & (BF16 ? (hi & 0xffff0000u) | (lo & 0xffffu) : hi);
                         }
-                if (odd) odd_s = 1;
+                }
+                if (fine != ~0u) odd_s = 1;
             }
 
             // ---- O^T += V^T P^T
@@ -485,31 +532,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
         }
     }
 
-    // Writes dims dd..dd+3 of row rr: O over the sum of weights, zeros where nothing
-    // was seen.
-    auto put = [&](int rr, int dd, vf4 x, float l) __attribute__((always_inline)) {
-        const int r = row0 + rr, t = quotient(r, p.by_g);
-        if (t >= count) return;
-        float* const out = p.o.p + b * p.o.sb + (h * p.G + r - t * p.G) * p.o.sh + t * p.o.st;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        x = l == 0.f ? vf4{0.f, 0.f, 0.f, 0.f} : x * inv;
-        if (p.vec_o) {
-            if (FULL || dd < pool.d) *reinterpret_cast<vf4*>(out + dd) = x;
-        } else {
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-                if (dd + i < pool.d) out[(dd + i) * p.o.sd] = x[0];
-                x = vf4{x[1], x[2], x[3], x[0]};
-            }
-        }
-    };
-
     // ---- the 4 waves' (m, l, O), one tile of rows at a time
     const int64_t rec_floats = paged_record_floats(p.rec_rows, D);
     const int o_at = (2 * p.rec_rows + 3) & ~3;          // O of a record
-    const int heads_blocks = pool.Hkv * p.n_rb;
-    const int64_t rec0 = ((int64_t)p.prefix[bl] * pool.Hkv + h) * p.n_rb + rb;   // part 0's record
-    const __amdgpu_buffer_rsrc_t rec_range = coherent_range(p.ws + (rec0 + (int64_t)part * heads_blocks) * rec_floats,
+    const __amdgpu_buffer_rsrc_t rec_range = coherent_range(p.ws + (parts.rec0 + part * parts.rec_step) * rec_floats,
                                                             live > 1 ? (uint32_t)rec_floats * 4u : 0u);
 #pragma unroll
     for (int rt = 0; rt < NRT; ++rt) {
@@ -527,8 +553,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
             ml_s[wave][col][1] = l_all;
         }
         __syncthreads();
-        for (int e = tid; e < 16 * (D / 4); e += 256) {
-            const int lr = e / (D / 4), dd = 4 * (e % (D / 4)), rr = 16 * rt + lr;
+        for (int f = tid; f < 16 * (D / 4); f += 256) {
+            const int lr = f / (D / 4), dd = 4 * (f % (D / 4)), rr = 16 * rt + lr;
             if (rr >= n_rows) continue;
             float M = kNegInf;
 #pragma unroll
@@ -542,7 +568,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
                 l += f * ml_s[w][lr][1];
                 acc += f * *reinterpret_cast<const vf4*>(ob + (w * 16 + lr) * OS + dd);
             }
-            if (odd_s) {                 // values that are not finite, for the rows that see them
+            if (DRAFT && odd_s) {        // values that are not finite, for the rows that see them
                 const int t = quotient(row0 + rr, p.by_g);
                 for (int key = max(k0, len); key < k1; ++key) {
                     const int row = paged_row(pool, table, h, key);
@@ -557,14 +583,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
                 }
             }
             if (live == 1) {
-                put(rr, dd, acc, l);
+                put_row4(p, b, h, row0 + rr, count, dd, acc, l);
             } else {
                 store_coherent4(rec_range, (uint32_t)(4 * (o_at + rr * D + dd)), acc);
                 if (dd == 0) store_coherent2(rec_range, (uint32_t)(8 * rr), M, l);
             }
         }
     }
-    if (live == 1) return;
+    if (live == 1 || !p.cnt) return;     // (without counters paged_combine_kernel merges)
 
     // ---- the last of the parts to arrive merges their records in order
     wait_stores_performed();
@@ -579,10 +605,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
     // all of them in flight (a trip to the coherence point is about 1.2 us: with 8
     // loads a trip the merge of 14 records of 32 rows took 13 us of a 26 us launch).
     constexpr int VPT = (ROWS * D / 4 + 255) / 256, EV = VPT < 4 ? VPT : 4, NR = (NRT == 1 ? 16 : 32) / EV;
-    const uint32_t step = (uint32_t)(heads_blocks * rec_floats * 4);     // bytes between two parts' records
-    const __amdgpu_buffer_rsrc_t range = coherent_range(p.ws + rec0 * rec_floats,
+    const uint32_t step = (uint32_t)(parts.rec_step * rec_floats * 4);     // bytes between two parts' records
+    const __amdgpu_buffer_rsrc_t range = coherent_range(p.ws + parts.rec0 * rec_floats,
                                                         (uint32_t)(live - 1) * step + (uint32_t)rec_floats * 4u);
-    for (int e0 = tid; e0 < n_rows * (D / 4); e0 += 256 * EV) {
+    for (int f0 = tid; f0 < n_rows * (D / 4); f0 += 256 * EV) {
         float M[EV], l[EV];
         vf4 acc[EV];
 #pragma unroll
@@ -598,8 +624,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
             for (int c = 0; c < NR; ++c)
 #pragma unroll
                 for (int v = 0; v < EV; ++v) {       // (past the last record: zeros, without an access)
-                    const int e = e0 + 256 * v, rr = e / (D / 4), dd = 4 * (e % (D / 4));
-                    const uint32_t at = e < n_rows * (D / 4) ? (uint32_t)(c0 + c) * step : 0xfffffff0u - 4u * ROWS * (D + 2);
+                    const int f = f0 + 256 * v, rr = f / (D / 4), dd = 4 * (f % (D / 4));
+                    const uint32_t at = f < n_rows * (D / 4) ? (uint32_t)(c0 + c) * step : 0xfffffff0u - 4u * ROWS * (D + 2);
                     ml[v][c] = load_coherent2(range, at + 8u * rr);
                     x[v][c] = load_coherent4(range, at + 4u * (o_at + rr * D + dd));
                 }
@@ -626,30 +652,88 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_attention_kernel(
         }
 #pragma unroll
         for (int v = 0; v < EV; ++v) {
-            const int e = e0 + 256 * v, rr = e / (D / 4), dd = 4 * (e % (D / 4));
-            if (rr < n_rows) put(rr, dd, acc[v], l[v]);
+            const int f = f0 + 256 * v, rr = f / (D / 4), dd = 4 * (f % (D / 4));
+            if (rr < n_rows) put_row4(p, b, h, row0 + rr, count, dd, acc[v], l[v]);
         }
     }
 }
 
-template <bool BF16, int D, int NRT, bool NT>
+// Merges the records of a (sequence, KV head, row block), in the order of the
+// parts: one thread per 4 dims of a row.  Behind launches whose merge is long:
+// records of many rows, which one workgroup would be reading for longer than a
+// launch takes.
+template <int D>
+__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnParams p, int tile_rows) {
+    int unit = blockIdx.x, rb = 0;
+    if (p.n_rb > 1) {
+        const int z = quotient(unit, p.by_rb);
+        rb = unit - z * p.n_rb;
+        unit = z;
+    }
+    const int bl = quotient(unit, p.by_hkv), h = unit - bl * p.pool.Hkv, b = p.b0 + bl;
+    const int ROUND = p.pool.bf16 ? 128 : 64, row0 = rb * tile_rows, n_rows = min(tile_rows, p.R - row0);
+    const int count = paged_count(p.counts, b, p.T), len = paged_len(p.pool, b);
+    const int n_keys = block_keys(p, row0, n_rows, len, count);
+    const Parts parts = even_parts(p, p.prefix[bl], p.prefix[bl + 1] - p.prefix[bl], h, rb, n_keys, ROUND);
+    const int f = blockIdx.y * 256 + threadIdx.x, rr = f / (D / 4), dd = 4 * (f % (D / 4));
+    if (parts.live <= 1 || rr >= n_rows) return;
+    const int64_t rec_floats = paged_record_floats(p.rec_rows, D), step = parts.rec_step * rec_floats;
+    const float* const rec = p.ws + parts.rec0 * rec_floats;
+    const int o_at = (2 * p.rec_rows + 3) & ~3;
+    constexpr int NR = 16;
+    float M = kNegInf, l = 0.f;
+    vf4 acc = vf4{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = 0; c0 < parts.live; c0 += NR) {
+        vf2 ml[NR];
+        vf4 x[NR];
+#pragma unroll
+        for (int c = 0; c < NR; ++c) {
+            const float* const at = rec + min(c0 + c, parts.live - 1) * step;
+            ml[c] = *reinterpret_cast<const vf2*>(at + 2 * rr);
+            x[c] = *reinterpret_cast<const vf4*>(at + o_at + rr * D + dd);
+        }
+        float M_new = M;
+#pragma unroll
+        for (int c = 0; c < NR; ++c) M_new = fmaxf(M_new, ml[c][0]);
+        const float M_use = M_new == kNegInf ? 0.f : M_new;
+        const float old = fast_exp2(M - M_use);
+        l *= old;
+        acc *= old;
+        M = M_new;
+#pragma unroll
+        for (int c = 0; c < NR; ++c) {
+            const float w = c0 + c < parts.live ? fast_exp2(ml[c][0] - M_use) : 0.f;
+            l += w * ml[c][1];
+            acc += w * x[c];
+        }
+    }
+    put_row4(p, b, h, row0 + rr, count, dd, acc, l);
+}
+
+template <bool BF16, int D, int NRT, bool NT, bool DRAFT>
 hipError_t launch_tile(const PagedAttnParams& p, hipStream_t stream) {
     const int64_t units = (int64_t)p.prefix[p.B] * p.pool.Hkv;
     const int64_t wgs = p.n_rb > 1 ? (units + 7) / 8 * 8 * p.n_rb : units;
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     if (p.pool.d == D)
-        hipLaunchKernelGGL((paged_attention_kernel<BF16, D, NRT, true, NT>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((paged_attention_kernel<BF16, D, NRT, true, NT, DRAFT>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
     else
-        hipLaunchKernelGGL((paged_attention_kernel<BF16, D, NRT, false, NT>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((paged_attention_kernel<BF16, D, NRT, false, NT, DRAFT>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !p.combine) return e;
+    const int64_t all = (int64_t)p.B * p.pool.Hkv * p.n_rb;
+    if (all > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(paged_combine_kernel<D>, dim3((unsigned)all, (p.rec_rows * D / 4 + 255) / 256), dim3(256), 0,
+                       stream, p, 16 * NRT);
     return hipGetLastError();
 }
 
 template <bool BF16, int D>
 hipError_t launch_dim(const PagedAttnParams& p, hipStream_t stream) {
     // (one row block: each byte of K and V is read by one workgroup)
-    if (p.tile_rows == 16)
-        return p.n_rb == 1 ? launch_tile<BF16, D, 1, true>(p, stream) : launch_tile<BF16, D, 1, false>(p, stream);
-    return launch_tile<BF16, D, 2, false>(p, stream);
+    if (p.tile_rows == 32) return launch_tile<BF16, D, 2, false, true>(p, stream);
+    if (p.T == 1 && p.n_rb == 1) return launch_tile<BF16, D, 1, true, false>(p, stream);
+    return launch_tile<BF16, D, 1, false, true>(p, stream);
 }
 
 template <bool BF16>

@@ -15,7 +15,7 @@ int64_t paged_max_records(int64_t B, int64_t units, int64_t record_bytes, int cu
     return n * record_bytes <= kPagedRecordBytes ? n : 0;
 }
 
-int paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
+int64_t paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
     const int64_t units = (int64_t)p.pool.Hkv * p.n_rb;    // workgroups of a part
     int64_t longest = 1, total = 0;
     for (int b = 0; b < p.B; ++b) {
@@ -45,10 +45,12 @@ int paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
         if (time < best) { best = time; best_len = len; }
         if (len == step) break;
     }
+    p.combine = 0;
     p.prefix[0] = 0;
     for (int b = 0; b < p.B; ++b)
         p.prefix[b + 1] = (uint16_t)(p.prefix[b] + std::max<int64_t>(1, (keys[b] + best_len - 1) / best_len));
-    return p.prefix[p.B];
+    if (p.prefix[p.B] == p.B) p.combine = 0;
+    return p.prefix[p.B] > p.B ? p.prefix[p.B] * units : 0;
 }
 
 }  // namespace nne
