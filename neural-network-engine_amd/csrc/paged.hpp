@@ -63,8 +63,7 @@ struct PagedAttnParams {
     uint16_t prefix[kPagedSeqs + 1];
 };
 
-// Rows of the tile that R query rows take, and its dims.
-inline int paged_tile_rows(int R) { return R <= 16 ? 16 : 32; }
+// Dims of the tile.
 inline int paged_tile_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // Floats of a record: (max, sum) of each row, then 16-byte aligned rows of O.
@@ -73,14 +72,16 @@ __host__ __device__
 #endif
 inline int64_t paged_record_floats(int rows, int D) { return ((2 * rows + 3) & ~3) + (int64_t)rows * D; }
 
-// Most records of a launch over B sequences of `units` (KV head, row block) pairs
-// each, on a device of `cus` CUs; 0 where it never splits (the records of so many
-// rows would pass kPagedRecordBytes).
+// Most bytes of records of a launch over B sequences of R query rows per KV head, on a
+// device of `cus` CUs; 0 where it never splits (they would pass kPagedRecordBytes).
 constexpr int64_t kPagedRecordBytes = int64_t{1} << 28;
-int64_t paged_max_records(int64_t B, int64_t units, int64_t record_bytes, int cus);
+int64_t paged_record_bytes(int64_t B, int64_t Hkv, int64_t R, int64_t d, int cus);
 
-// Fills p.prefix and p.combine for sequences of keys[b] keys (p's sizes set);
-// returns the number of records (0: nothing is split).
+// Tiles of 16 or 32 rows: sets tile_rows, n_rb, by_rb and rec_rows of p.
+void paged_set_tile(PagedAttnParams& p, int tile_rows);
+
+// Takes the tile and fills p.prefix and p.combine for sequences of keys[b] keys (p's
+// sizes set); returns the number of records (0: nothing is split).
 int64_t paged_plan(PagedAttnParams& p, const int64_t* keys, int cus);
 
 struct PagedAppendParams {

@@ -156,12 +156,6 @@ int check_positions(const int32_t* start, const int32_t* depths_dev, const int32
     return NNE_OK;
 }
 
-// Workgroups of a part, per KV head of the cache.
-int64_t row_blocks(int64_t R) {
-    const int tile = nne::paged_tile_rows((int)R);
-    return (R + tile - 1) / tile;
-}
-
 int check_attention_heads(const nne_paged_cache_t* c, int64_t Hq, int64_t T) {
     if (Hq <= 0 || Hq > INT32_MAX || Hq % c->Hkv != 0)
         return fail_format(NNE_EINVAL, NNE_BAD "num_heads (%lld) must be divisible by num_kv_heads (%lld) for GQA",
@@ -173,15 +167,13 @@ int check_attention_heads(const nne_paged_cache_t* c, int64_t Hq, int64_t T) {
 
 // Workspace of launches over the batch's groups of sequences, with T tokens.
 nne_workspace_size_t attention_size(const nne_paged_cache_t* c, int64_t Hq, int64_t T) {
-    const int64_t R = Hq / c->Hkv * T, units = c->Hkv * row_blocks(R);
-    const int64_t rec = 4 * nne::paged_record_floats((int)std::min<int64_t>(R, nne::paged_tile_rows((int)R)),
-                                                     nne::paged_tile_dim((int)c->d));
+    const int64_t R = Hq / c->Hkv * T;
     const int64_t group = std::min<int64_t>(c->B, nne::kPagedSeqs), rest = c->B % nne::kPagedSeqs;
     const int cus = nne::cus_of_device();
     nne_workspace_size_t s;
-    s.records_bytes = (uint64_t)(rec * std::max(nne::paged_max_records(group, units, rec, cus),
-                                                rest ? nne::paged_max_records(rest, units, rec, cus) : 0));
-    s.n_counters = (uint64_t)std::max<int64_t>(group * units, c->B);
+    s.records_bytes = (uint64_t)std::max(nne::paged_record_bytes(group, c->Hkv, R, c->d, cus),
+                                         rest ? nne::paged_record_bytes(rest, c->Hkv, R, c->d, cus) : 0);
+    s.n_counters = (uint64_t)std::max<int64_t>(group * c->Hkv * ((R + 15) / 16), c->B);
     return s;
 }
 
@@ -372,16 +364,11 @@ int nne_paged_attention(const nne_paged_cache_t* cache, const float* q, const in
     p.G = (int)(Hq / cache->Hkv);
     p.T = (int)T;
     p.R = p.G * p.T;
-    p.tile_rows = nne::paged_tile_rows(p.R);
-    p.n_rb = (int)row_blocks(p.R);
     p.by_g = nne::divisor(p.G);
     p.by_hkv = nne::divisor(p.pool.Hkv);
-    p.by_rb = nne::divisor(p.n_rb);
-    p.rec_rows = std::min(p.R, p.tile_rows);
     p.vec_q = vec_view(q, qs.v);
     p.vec_o = vec_view(o, os.v);
     p.qscale = (has_scale ? scale : 1.0f / std::sqrt((float)d)) * nne::kLog2e;
-    const int64_t rec_bytes = 4 * nne::paged_record_floats(p.rec_rows, nne::paged_tile_dim((int)d));
     const hipStream_t s = static_cast<hipStream_t>(stream);
     // Launches of up to kPagedSeqs sequences, in stream order on one workspace.
     for (int64_t b0 = 0; b0 < B; b0 += nne::kPagedSeqs) {
@@ -397,6 +384,7 @@ int nne_paged_attention(const nne_paged_cache_t* cache, const float* q, const in
         p.cnt = nullptr;
         if (n_records > 0) {
             void* records = nullptr;
+            const int64_t rec_bytes = 4 * nne::paged_record_floats(p.rec_rows, nne::paged_tile_dim((int)d));
             rc = nne::take_workspace(ws, (uint64_t)(n_records * rec_bytes),
                                      p.combine ? 0 : (int64_t)p.B * p.pool.Hkv * p.n_rb, s, &records, &p.cnt,
                                      "paged attention");

@@ -402,6 +402,15 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attent
                             s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qv[i], s[rt][0], 0, 0, 0);
                     }
                 }
+            // Q two steps ahead of the products: read where it is used, each step
+            // waited for the LDS.
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * S::QP, 0);
+#pragma unroll
+            for (int i = 0; i < KS * NRT - 2; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, BF16 ? 3 * KT : 4, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, S::QP, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, BF16 ? 6 * KT : 8, 0);
             const bool more = blk + 4 < n_blocks;
             if (more) load_k(blk + 4);
 

@@ -1,56 +1,118 @@
-// Key split of the paged-attention kernel: how many workgroups share a
-// (sequence, KV head, row block).
+// Rows of the tile and key split of the paged-attention kernel: how many workgroups
+// share a sequence's rows and keys.
 #include <algorithm>
+#include <cmath>
 
 #include "paged.hpp"
 
 namespace nne {
 
 namespace {
+
 constexpr int kTargetPerCu = 4;    // workgroups per CU that a split may make
+
+// Times of the kernel, fitted to 2200 launches of 60 shapes (1-62 sequences of 5-8000
+// keys, 1-256 rows, head dims 64-256, both types, parts of 128-8448 keys; rms error of
+// the fit 8 %; the part length it picks is 1.2 % above the best of those timed).
+// Rows: tiles of 16 and of 32 rows; columns: f32 and bf16 pools.
+constexpr float kStart[2][2] = {{0.f, 1.0f}, {0.6f, 4.4f}};         // us of a workgroup
+constexpr float kStartDims[2][2] = {{2.8f, 1.5f}, {3.8f, 1.7f}};    // and per 128 dims
+constexpr float kKey[2][2] = {{.0063f, .0051f}, {0.f, 0.f}};        // us of a key
+constexpr float kKeyDims[2][2] = {{.0148f, .0055f}, {.0325f, .0148f}};
+constexpr float kAtOnce[2][2] = {{1.14f, 1.08f}, {1.05f, 1.40f}};   // gain of several on a CU
+constexpr float kBytesPerUs = 5.76e6f;
+constexpr float kMerge = 0.8f, kMergePart = .072f, kMergeFloat = 1.04e-4f;   // by the last to arrive
+constexpr float kCombine = 3.7f, kCombinePart = .042f;                       // by a launch of its own
+
+// Sum of the fourth powers' root: the largest of the three, with the overlap of
+// those that come near it.
+float joined(float a, float b, float c) {
+    a *= a, b *= b, c *= c;
+    return std::sqrt(std::sqrt(a * a + b * b + c * c));
 }
 
-int64_t paged_max_records(int64_t B, int64_t units, int64_t record_bytes, int cus) {
-    const int64_t n = (int64_t)kTargetPerCu * cus + B * units;
-    return n * record_bytes <= kPagedRecordBytes ? n : 0;
+// Upwards to a whole number (conversions, which vectorise where ceil is a call).
+float up(float x) { return (float)(int)(std::min(x, 1e9f) + .9999f); }
+
+}  // namespace
+
+int64_t paged_record_bytes(int64_t B, int64_t Hkv, int64_t R, int64_t d, int cus) {
+    const int64_t n = (int64_t)kTargetPerCu * cus + B * Hkv * ((R + 31) / 32);
+    const int64_t record = 4 * paged_record_floats((int)std::min<int64_t>(R, 32), paged_tile_dim((int)d));
+    return n <= kPagedRecordBytes / record ? n * record : 0;
+}
+
+void paged_set_tile(PagedAttnParams& p, int tile_rows) {
+    p.tile_rows = tile_rows;
+    p.n_rb = (p.R + tile_rows - 1) / tile_rows;
+    p.by_rb = divisor(p.n_rb);
+    p.rec_rows = std::min(p.R, tile_rows);
 }
 
 int64_t paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
-    const int64_t units = (int64_t)p.pool.Hkv * p.n_rb;    // workgroups of a part
-    int64_t longest = 1, total = 0;
-    for (int b = 0; b < p.B; ++b) {
-        longest = std::max(longest, keys[b]);
-        total += keys[b];
-    }
-    // Part lengths from the longest sequence down to 64 keys; the one of least
-    // modelled time: a workgroup pays a fixed time and its keys, as many run at
-    // once as the device holds, and a sequence in parts pays their merge.
+    const int D = paged_tile_dim(p.pool.d), type = p.pool.bf16 ? 1 : 0;
     const int64_t step = p.pool.bf16 ? 128 : 64;           // keys of a round of the waves
-    const int64_t slots = 2 * (int64_t)cus;
-    const int64_t most = paged_max_records(p.B, units, 4 * paged_record_floats(p.rec_rows, paged_tile_dim(p.pool.d)), cus);
-    int64_t best_len = longest;
-    double best = 1e300;
-    for (int64_t n = 1; n <= 512; n = n < 8 ? n + 1 : n + n / 4) {
-        const int64_t len = ((longest + n - 1) / n + step - 1) / step * step;
-        int64_t parts = 0;
-        for (int b = 0; b < p.B; ++b) parts += std::max<int64_t>(1, (keys[b] + len - 1) / len);
-        const int64_t wgs = parts * units;
-        if (n > 1 && wgs > most) break;
-        const int64_t rounds = (wgs + slots - 1) / slots;
-        // Long launches flow through the device, short ones run in rounds.
-        const double flow = (double)total * units / slots;
-        const double time = 400.0 + (rounds <= 2 ? (double)rounds * (double)(std::min(len, longest) + 150)
-                                                 : flow + 150.0 * rounds + 0.5 * (double)len)
-                            + (n > 1 ? 100.0 + 12.0 * (double)n : 0.0);
-        if (time < best) { best = time; best_len = len; }
-        if (len == step) break;
+    const int64_t most_bytes = paged_record_bytes(p.B, p.pool.Hkv, p.R, p.pool.d, cus);
+    float rounds[kPagedSeqs], longest = 1.f, total = 0.f, sum = 0.f;
+    for (int b = 0; b < p.B; ++b) {
+        rounds[b] = (float)((keys[b] + step - 1) / step);
+        longest = std::max(longest, rounds[b]);
+        total += rounds[b];
+        sum += (float)keys[b];
     }
-    p.combine = 0;
+    const float memory = sum * (float)(p.pool.Hkv * p.pool.d * (p.pool.bf16 ? 4 : 8)) / kBytesPerUs;
+    // Tiles of 16 rows start sooner and spread few rows over more CUs, tiles of 32
+    // bring K and V half as often: 52 rows of a sequence of 1746 keys take 16.3 and
+    // 18.6 us, 256 rows of 8 sequences of 1024-4160 keys 127 and 86.  The part length
+    // and the tile of least modelled time: a workgroup pays a fixed time and its
+    // keys, a CU its share of them, the memory the bytes, and parts pay their merge.
+    int best_tile = 16, best_combine = 0;
+    float best = 1e30f, best_rounds = longest;
+    for (int tile = 16; tile <= (p.R > 16 ? 32 : 16); tile += 16) {
+        const int at = tile / 32, rows = std::min(p.R, tile);
+        const float units = (float)p.pool.Hkv * (float)((p.R + tile - 1) / tile);   // workgroups of a part
+        const float start = kStart[at][type] + kStartDims[at][type] * (float)D / 128.f;
+        const float key = kKey[at][type] + kKeyDims[at][type] * (float)D / 128.f;
+        const float record = 4.f * (float)paged_record_floats(rows, D);
+        float last = 0.f;
+        for (int n = 1; n <= 512; n = n < 8 ? n + 1 : n + n / 4) {
+            const float len = up(longest / (float)n), inv = 1.f / len;
+            if (len == last) continue;
+            last = len;
+            float parts = 0.f;
+            for (int b = 0; b < p.B; ++b) parts += std::max(1.f, up(rounds[b] * inv));
+            const float wgs = parts * units;
+            if (n > 1 && wgs * record > (float)most_bytes) break;
+            const float one = start + key * len * (float)step;
+            const float mean = start + key * total * units / wgs * (float)step;
+            const float share = up(wgs / (float)cus) * mean / kAtOnce[at][type];
+            float time = joined(one, share, memory);
+            int combine = 0;
+            if (n > 1) {
+                const float merge = kMerge + (float)n * (kMergePart + kMergeFloat * (float)(rows * D));
+                const float launch = kCombine + (float)n * kCombinePart;
+                combine = launch < merge;
+                time += std::min(merge, launch);
+            }
+            if (time < best) best = time, best_rounds = len, best_tile = tile, best_combine = combine;
+            if (len == 1.f) break;
+        }
+    }
+    paged_set_tile(p, best_tile);
+    const int64_t units = (int64_t)p.pool.Hkv * p.n_rb, best_len = (int64_t)best_rounds * step;
+    const int64_t record = 4 * paged_record_floats(p.rec_rows, D);
+    int64_t parts = 0;
     p.prefix[0] = 0;
-    for (int b = 0; b < p.B; ++b)
-        p.prefix[b + 1] = (uint16_t)(p.prefix[b] + std::max<int64_t>(1, (keys[b] + best_len - 1) / best_len));
-    if (p.prefix[p.B] == p.B) p.combine = 0;
-    return p.prefix[p.B] > p.B ? p.prefix[p.B] * units : 0;
+    for (int b = 0; b < p.B; ++b) {
+        parts += std::max<int64_t>(1, (keys[b] + best_len - 1) / best_len);
+        p.prefix[b + 1] = (uint16_t)parts;
+    }
+    if (parts > p.B && (parts > UINT16_MAX || parts * units * record > most_bytes)) {   // (a rounding of the model's)
+        parts = p.B;
+        for (int b = 0; b < p.B; ++b) p.prefix[b + 1] = (uint16_t)(b + 1);
+    }
+    p.combine = parts > p.B ? best_combine : 0;
+    return parts > p.B ? parts * units : 0;
 }
 
 }  // namespace nne
