@@ -448,7 +448,10 @@ int nne_paged_workspace_size(const nne_paged_cache_t *cache, int64_t Hq, int64_t
  * layer_stride elements behind.  NULL paths: the first counts[b] tokens as
  * they lie.  NULL counts_dev: counts_host[0] for every sequence, and the call
  * needs no device array.  ws as for nne_paged_attention (counters only).
- * NNE_EINVAL (nothing moved) for paths that do not ascend or leave the pages. */
+ * NNE_EINVAL (nothing moved) for paths that do not ascend or leave the pages,
+ * and with table_host where a page would take rows of two sequences.  lens_host
+ * advances with the call: after replays of a captured one, set it from the
+ * device's before the next call. */
 int nne_paged_commit(const nne_paged_cache_t *cache, int64_t n_layers, int64_t layer_stride,
                      const int32_t *counts_dev, const int32_t *counts_host,
                      const int32_t *paths_dev, const int32_t *paths_host, int64_t J,

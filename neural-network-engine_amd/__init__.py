@@ -778,7 +778,7 @@ def _check_f32(index, *ts):
         if t.dtype is not f32 or t.get_device() != index or index < 0:
             raise InvalidArgument("Invalid configuration or argument: expected float32 tensors on GPU "
                                   "%d, got %s on %s" % (index, t.dtype, t.device))
-    if _torch._C._cuda_getDevice() != index:
+    if index < 0 or _torch._C._cuda_getDevice() != index:
         raise InvalidArgument("Invalid configuration or argument: GPU %d is not the current device"
                               % index)
 

@@ -106,6 +106,27 @@ int check_pages(const nne_paged_cache_t* c, int64_t b, int64_t first, int64_t en
     return NNE_OK;
 }
 
+// The same, and the pages go to `pages`: those that take new rows.
+int add_pages(const nne_paged_cache_t* c, int64_t b, int64_t first, int64_t end, std::vector<int32_t>& pages) {
+    const int rc = check_pages(c, b, first, end);
+    if (rc || !c->table_host || first >= end) return rc;
+    const int32_t* t = c->table_host + b * c->max_pages;
+    try {
+        pages.insert(pages.end(), t + first / c->page_size, t + (end - 1) / c->page_size + 1);
+    } catch (const std::bad_alloc&) {
+        return fail_format(NNE_EINVAL, NNE_BAD "out of host memory");
+    }
+    return NNE_OK;
+}
+
+// No page takes new rows of two sequences (or through two entries of one).
+int check_apart(std::vector<int32_t>& pages) {
+    std::sort(pages.begin(), pages.end());
+    const auto twice = std::adjacent_find(pages.begin(), pages.end());
+    if (twice == pages.end()) return NNE_OK;
+    return fail_format(NNE_EINVAL, NNE_BAD "page %d would take new rows of two places", *twice);
+}
+
 nne::PagedPool make_pool(const nne_paged_cache_t* c) {
     nne::PagedPool p{};
     p.k = c->k;
@@ -254,7 +275,7 @@ int nne_paged_append(const nne_paged_cache_t* cache, const float* k_new, const i
     if (rc == NNE_OK) rc = check_room(cache, T, counts_host, NNE_ECAPACITY);
     if (rc == NNE_OK) rc = check_rotation(cos_table, sin_table, max_seq_len, table_head_dim, cache->d);
     if (rc) return rc;
-    const int64_t B = cache->B, P = cache->page_size;
+    const int64_t B = cache->B;
     if (B > INT32_MAX / std::max<int64_t>(T, 1))
         return fail_format(NNE_EINVAL, NNE_BAD "%lld tokens of %lld sequences", (long long)T, (long long)B);
     if (B == 0 || T == 0) return NNE_OK;
@@ -263,25 +284,11 @@ int nne_paged_append(const nne_paged_cache_t* cache, const float* k_new, const i
         if (rc) return rc;
     }
     if (cache->table_host) {
-        // Every new row has a page, and no page is written by two sequences (or
-        // through two entries of one).
         std::vector<int32_t> pages;
-        try {
-            for (int64_t b = 0; b < B; ++b) {
-                const int64_t first = cache->lens_host[b], end = first + count_of(counts_host, b, T);
-                rc = check_pages(cache, b, first, end);
-                if (rc) return rc;
-                if (first < end)
-                    pages.insert(pages.end(), cache->table_host + b * cache->max_pages + first / P,
-                                 cache->table_host + b * cache->max_pages + (end - 1) / P + 1);
-            }
-        } catch (const std::bad_alloc&) {
-            return fail_format(NNE_EINVAL, NNE_BAD "out of host memory");
-        }
-        std::sort(pages.begin(), pages.end());
-        const auto twice = std::adjacent_find(pages.begin(), pages.end());
-        if (twice != pages.end())
-            return fail_format(NNE_EINVAL, NNE_BAD "page %d would take new rows of two places", *twice);
+        for (int64_t b = 0; b < B && rc == NNE_OK; ++b)
+            rc = add_pages(cache, b, cache->lens_host[b], cache->lens_host[b] + count_of(counts_host, b, T), pages);
+        if (rc == NNE_OK) rc = check_apart(pages);
+        if (rc) return rc;
     }
     if (!k_new || !v_new) return fail_format(NNE_EINVAL, NNE_BAD "null tensor pointer");
     rc = check_device_side(cache);
@@ -412,6 +419,7 @@ int nne_paged_commit(const nne_paged_cache_t* cache, int64_t n_layers, int64_t l
     if (!counts_host) return fail_format(NNE_EINVAL, NNE_BAD "counts_host is null");
     if (!paths_dev != !paths_host)
         return fail_format(NNE_EINVAL, NNE_BAD "paths are needed on the device and on the host");
+    std::vector<int32_t> pages;
     for (int64_t b = 0; b < B; ++b) {
         const int64_t n = counts_dev ? counts_host[b] : counts_host[0];
         const int64_t len = cache->lens_host[b];
@@ -430,9 +438,11 @@ int nne_paged_commit(const nne_paged_cache_t* cache, int64_t n_layers, int64_t l
             return fail_format(NNE_EINVAL, NNE_BAD "row %lld of sequence %lld is past its %lld pages of %lld rows",
                                (long long)(len + last), (long long)b, (long long)cache->max_pages,
                                (long long)cache->page_size);
-        rc = check_pages(cache, b, len, len + last + 1);
+        rc = paths_host ? add_pages(cache, b, len, len + last + 1, pages) : check_pages(cache, b, len, len + last + 1);
         if (rc) return rc;
     }
+    rc = check_apart(pages);
+    if (rc) return rc;
     if (J == 0) return NNE_OK;
     rc = check_device_side(cache);
     if (rc) return rc;
