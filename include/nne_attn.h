@@ -414,7 +414,7 @@ int nne_qk_norm_rope(const float *q, const int64_t q_shape[4], const int64_t q_s
  * advances it, and until then another call writes the same rows again.
  * NNE_ECAPACITY (nothing written) if a sequence has no room for its rows in
  * max_pages pages; with table_host NNE_EINVAL if a row has no page or two
- * sequences would write one page. */
+ * sequences would write one page, and for 2^34 values of k_new or more. */
 int nne_paged_append(const nne_paged_cache_t *cache, const float *k_new,
                      const int64_t k_new_strides[4], const float *v_new,
                      const int64_t v_new_strides[4], int64_t T, const int32_t *counts_dev,

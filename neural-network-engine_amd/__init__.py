@@ -915,13 +915,16 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6
     k=None: q alone.  Returns (q_out, k_out): new tensors in the inputs' order of dims
     by default, or the given ones (q and k themselves are fine)."""
     qs, index = q.shape, q.get_device()
-    _check_f32(index, *[t for t in (q, k, q_weight, k_weight) if t is not None])
+    if k is None or q_weight is None or k_weight is None:
+        _check_f32(index, *[t for t in (q, k, q_weight, k_weight) if t is not None])
+    else:
+        _check_f32(index, q, k, q_weight, k_weight)
     if len(qs) != 4 or (k is not None and k.dim() != 4):
         _shape4(q, "Q")
         _shape4(k, "K")
     b, _, t, d = qs
     for w in (q_weight, k_weight):
-        if w is not None and (w.dim() != 1 or w.numel() != d or not w.is_contiguous()):
+        if w is not None and (w.shape != (d,) or not w.is_contiguous()):
             raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
                                 % ([d], list(w.shape)))
     if q_out is None:

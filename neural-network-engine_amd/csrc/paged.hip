@@ -4,6 +4,7 @@
 // and by latency where they are short; each is one launch that reads and writes
 // every value once.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_device.hpp"
 #include "paged_launch.hpp"
@@ -56,12 +57,12 @@ __device__ __forceinline__ void store_row4(void* pool, int64_t at, vf4 x) {
 template <bool BF16>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendParams p) {
     const int per_row = p.pool.d / 8, per_token = per_row * p.pool.Hkv;
-    const int64_t n = (int64_t)p.B * p.T * per_token;
+    const uint32_t n = (uint32_t)p.B * p.T * per_token;       // (the host keeps this in 31 bits)
     const int half = p.pool.d / 2;
-    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += gridDim.x * 256ll) {
-        const int token = (int)(e / per_token), in = (int)(e % per_token);
-        const int h = in / per_row, i = 4 * (in % per_row);
-        const int b = token / p.T, t = token % p.T;
+    for (uint32_t e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
+        const int token = quotient(e, p.by_token), in = e - token * per_token;
+        const int h = quotient(in, p.by_row), i = 4 * (in - h * per_row);
+        const int b = quotient(token, p.by_t), t = token - b * p.T;
         const float* kr = p.k.p + b * p.k.sb + h * p.k.sh + t * p.k.st;
         const float* vr = p.v.p + b * p.v.sb + h * p.v.sh + t * p.v.st;
         const bool vec = p.vec != 0;
@@ -97,10 +98,10 @@ constexpr int kCommitStage = 256;  // path entries in LDS at a time
 // (each lookup is a chain of two loads: eight in a row, one after the other in
 // every thread, took most of the kernel's time), and the last of its workgroups
 // to have read lens advances it.  Bound by memory: 32 layers of 8 heads of 16
-// sequences, 4.5 rows in the mean, are 38 MB read and written.
+// sequences, 4.5 rows in the mean, are 19 MB read and written in pieces of 256 bytes
+// all over the pools, 11.6 us.
 __global__ __launch_bounds__(256) void paged_commit_kernel(const PagedCommitParams p) {
     __shared__ int from_s[kCommitStage], to_s[kCommitStage];
-    __shared__ int last;
     const int b = blockIdx.y, tid = threadIdx.x;
     const PagedPool& c = p.pool;
     const int32_t* table = c.table + (int64_t)b * c.max_pages;
@@ -117,6 +118,7 @@ __global__ __launch_bounds__(256) void paged_commit_kernel(const PagedCommitPara
     char* const at = static_cast<char*>(rest >= c.Hkv * vecs ? c.v : c.k) + layer * p.layer_stride +
                      (int64_t)h * c.page_size * row_bytes + 16 * (rest % vecs);
     const bool mine = layer < p.n_layers;
+    uint32_t arrived = 0;
     for (int j0 = 0; j0 < count; j0 += kCommitStage) {
         const int n = min(kCommitStage, count - j0);
         if (j0 > 0) {
@@ -132,28 +134,32 @@ __global__ __launch_bounds__(256) void paged_commit_kernel(const PagedCommitPara
         from_s[tid] = to < 0 ? -1 : from;
         to_s[tid] = from < 0 ? -1 : to;
         __syncthreads();
+        // Every thread of the workgroup has its len: it has arrived (the answer comes
+        // while rows move).
+        if (j0 == 0 && tid == 0)
+            arrived = __hip_atomic_fetch_add(p.cnt + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         for (int j = 0; mine && j < n; j += kCommitRows) {
             vf4 val[kCommitRows];
+            int from8[kCommitRows], to8[kCommitRows];
 #pragma unroll
             for (int i = 0; i < kCommitRows; ++i) {   // (kCommitRows divides kCommitStage)
-                const int r = from_s[j + i];
-                if (r >= 0) val[i] = *reinterpret_cast<const vf4*>(at + r * row_bytes);
+                from8[i] = __builtin_amdgcn_readfirstlane(from_s[j + i]);
+                to8[i] = __builtin_amdgcn_readfirstlane(to_s[j + i]);
             }
 #pragma unroll
-            for (int i = 0; i < kCommitRows; ++i) {
-                const int r = to_s[j + i];
-                if (r >= 0) *reinterpret_cast<vf4*>(at + r * row_bytes) = val[i];
-            }
+            for (int i = 0; i < kCommitRows; ++i)
+                if (from8[i] >= 0) val[i] = *reinterpret_cast<const vf4*>(at + from8[i] * row_bytes);
+#pragma unroll
+            for (int i = 0; i < kCommitRows; ++i)
+                if (to8[i] >= 0) *reinterpret_cast<vf4*>(at + to8[i] * row_bytes) = val[i];
         }
     }
-    __syncthreads();                     // every thread has its len
-    if (tid == 0)
-        last = __hip_atomic_fetch_add(p.cnt + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-               gridDim.x - 1;
-    __syncthreads();
-    if (last && tid == 0) {
-        p.pool.lens[b] = min(len + count, c.max_pages * c.page_size);
-        __hip_atomic_store(p.cnt + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) {
+        if (count == 0) arrived = __hip_atomic_fetch_add(p.cnt + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (arrived == gridDim.x - 1) {
+            p.pool.lens[b] = min(len + count, c.max_pages * c.page_size);
+            __hip_atomic_store(p.cnt + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
 }
 
@@ -174,17 +180,20 @@ __device__ __forceinline__ int64_t norm_table_row(const NormRopeParams& p, int b
 
 // LPR lanes hold a head, 4 dims of each half per lane, so both values of a
 // rotated pair are in one lane; the sum of squares takes log2(LPR) lane
-// exchanges.  A head is read once and written once.
-template <int LPR>
+// exchanges.  A head is read once and written once, and the memory bounds a long
+// launch.  STREAM: the outputs are more than the L2s hold, and pass them by.  4
+// sequences of 1999 tokens of 32 + 8 heads of 64 dims, 164 MB: 29 us (5.6 TB/s),
+// 33 us without; 32 single tokens of 32 + 8 heads of 128 dims: 3.7 us.
+template <int LPR, bool STREAM>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NormRopeParams p) {
     const int heads = p.H[0] + p.H[1], half = p.d / 2;
-    const int64_t n = (int64_t)p.B * p.T * heads;
+    const uint32_t n = (uint32_t)p.B * p.T * heads;           // (the host keeps this in 31 bits)
     const int i = 4 * (threadIdx.x % LPR);
     const bool in = i < half;
-    for (int64_t r = (blockIdx.x * 256ll + threadIdx.x) / LPR; r < n; r += gridDim.x * (256ll / LPR)) {
-        const int token = (int)(r / heads);
-        int h = (int)(r % heads);
-        const int b = token / p.T, t = token % p.T;
+    for (uint32_t r = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; r < n; r += gridDim.x * (256 / LPR)) {
+        const int token = quotient(r, p.by_heads);
+        int h = r - token * heads;
+        const int b = quotient(token, p.by_t), t = token - b * p.T;
         const int which = h >= p.H[0];
         if (which) h -= p.H[0];
         const View4 x = which ? p.x[1] : p.x[0];
@@ -194,6 +203,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NormRopeParams 
             y0 = *reinterpret_cast<const vf4*>(row + i);
             y1 = *reinterpret_cast<const vf4*>(row + i + half);
         }
+        const int64_t tab = p.cos ? norm_table_row(p, b, t) : 0;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum += y0[j] * y0[j] + y1[j] * y1[j];
@@ -205,14 +215,16 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NormRopeParams 
         const vf4 one = vf4{1.f, 1.f, 1.f, 1.f};
         y0 = y0 * scale * (w ? *reinterpret_cast<const vf4*>(w + i) : one);
         y1 = y1 * scale * (w ? *reinterpret_cast<const vf4*>(w + i + half) : one);
-        if (p.cos) {
-            const int64_t at = norm_table_row(p, b, t);
-            rotate4(y0, y1, p.cos + at, p.sin + at, i, half);
-        }
+        if (p.cos) rotate4(y0, y1, p.cos + tab, p.sin + tab, i, half);
         const OutView4 o = which ? p.o[1] : p.o[0];
         float* out = o.p + b * o.sb + h * o.sh + t * o.st;
-        *reinterpret_cast<vf4*>(out + i) = y0;
-        *reinterpret_cast<vf4*>(out + i + half) = y1;
+        if constexpr (STREAM) {
+            __builtin_nontemporal_store(y0, reinterpret_cast<vf4*>(out + i));
+            __builtin_nontemporal_store(y1, reinterpret_cast<vf4*>(out + i + half));
+        } else {
+            *reinterpret_cast<vf4*>(out + i) = y0;
+            *reinterpret_cast<vf4*>(out + i + half) = y1;
+        }
     }
 }
 
@@ -250,6 +262,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(const NormRopePar
         }
     }
 }
+
+constexpr int64_t kL2Bytes = int64_t{32} << 20;   // the L2s of 8 XCDs
 
 unsigned grid_for(int64_t threads, int64_t most) {
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, most));
@@ -293,17 +307,21 @@ hipError_t launch_qk_norm_rope(const NormRopeParams& p, hipStream_t stream) {
     const int64_t n = (int64_t)p.B * p.T * (p.H[0] + p.H[1]);
     if (n <= 0) return hipSuccess;
     const int64_t most = 1 << 20;
-    if (!p.vec) {
+    if (!p.vec || n > INT32_MAX) {
         hipLaunchKernelGGL(qk_norm_rope_any_kernel, dim3(grid_for(n * 64, most)), dim3(256), 0, stream, p);
-    } else if (p.d <= 64) {
-        hipLaunchKernelGGL(qk_norm_rope_kernel<8>, dim3(grid_for(n * 8, most)), dim3(256), 0, stream, p);
-    } else if (p.d <= 128) {
-        hipLaunchKernelGGL(qk_norm_rope_kernel<16>, dim3(grid_for(n * 16, most)), dim3(256), 0, stream, p);
-    } else if (p.d <= 256) {
-        hipLaunchKernelGGL(qk_norm_rope_kernel<32>, dim3(grid_for(n * 32, most)), dim3(256), 0, stream, p);
-    } else {
-        hipLaunchKernelGGL(qk_norm_rope_kernel<64>, dim3(grid_for(n * 64, most)), dim3(256), 0, stream, p);
+        return hipGetLastError();
     }
+    const bool streams = n * p.d * 4 > kL2Bytes;
+    const auto launch = [&](auto lpr) {
+        constexpr int LPR = decltype(lpr)::value;
+        const dim3 grid(grid_for(n * LPR, most));
+        if (streams) hipLaunchKernelGGL((qk_norm_rope_kernel<LPR, true>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((qk_norm_rope_kernel<LPR, false>), grid, dim3(256), 0, stream, p);
+    };
+    if (p.d <= 64) launch(std::integral_constant<int, 8>());
+    else if (p.d <= 128) launch(std::integral_constant<int, 16>());
+    else if (p.d <= 256) launch(std::integral_constant<int, 32>());
+    else launch(std::integral_constant<int, 64>());
     return hipGetLastError();
 }
 

@@ -91,6 +91,7 @@ struct PagedAppendParams {
     const float *cos, *sin;    // null: no rotation
     int max_seq_len;
     int B, T;
+    Divisor by_token, by_row, by_t;       // threads of a token and of a row, T
     int vec;                   // k and v rows are 16-byte vectors
 };
 
@@ -109,6 +110,7 @@ struct NormRopeParams {
     const float* w[2];         // or null: ones
     int H[2];
     int B, T, d;
+    Divisor by_heads, by_t;
     int norm;
     float eps;
     const float *cos, *sin;    // null: no rotation

@@ -251,6 +251,8 @@ int nne_qk_norm_rope(const float* q, const int64_t q_shape[4], const int64_t q_s
     p.B = (int)B;
     p.T = (int)T;
     p.d = (int)d;
+    p.by_heads = nne::divisor(Hq + Hk);
+    p.by_t = nne::divisor(T);
     p.norm = has_norm != 0;
     p.eps = eps;
     p.cos = cos_table;
@@ -276,8 +278,10 @@ int nne_paged_append(const nne_paged_cache_t* cache, const float* k_new, const i
     if (rc == NNE_OK) rc = check_rotation(cos_table, sin_table, max_seq_len, table_head_dim, cache->d);
     if (rc) return rc;
     const int64_t B = cache->B;
-    if (B > INT32_MAX / std::max<int64_t>(T, 1))
-        return fail_format(NNE_EINVAL, NNE_BAD "%lld tokens of %lld sequences", (long long)T, (long long)B);
+    const int64_t per_token = cache->Hkv * (cache->d / 8);
+    if (B > 0 && T > INT32_MAX / B / per_token)
+        return fail_format(NNE_EINVAL, NNE_BAD "%lld tokens of %lld sequences: K may have 2^34 values", (long long)T,
+                           (long long)B);
     if (B == 0 || T == 0) return NNE_OK;
     if (cos_table) {
         rc = check_positions(cache->lens_host, depths_dev, depths_host, counts_host, B, T, max_seq_len);
@@ -305,6 +309,9 @@ int nne_paged_append(const nne_paged_cache_t* cache, const float* k_new, const i
     p.max_seq_len = (int)max_seq_len;
     p.B = (int)B;
     p.T = (int)T;
+    p.by_token = nne::divisor(cache->Hkv * (cache->d / 8));
+    p.by_row = nne::divisor(cache->d / 8);
+    p.by_t = nne::divisor(T);
     p.vec = vec_view(k_new, ks.v) && vec_view(v_new, vs.v);
     if (cos_table && (!aligned16(cos_table) || !aligned16(sin_table)))
         return fail_format(NNE_EINVAL, NNE_BAD "RoPE tables must be 16-byte aligned");

@@ -130,6 +130,26 @@ def test_serving_loop(nne, cuda, dtype, hq, hkv, d, page):
         assert np.array_equal(cache.lens_dev.cpu().numpy(), lens)
 
 
+@pytest.mark.parametrize("d,t", [(128, 701), (64, 1999)])
+def test_norm_rope_of_long_inputs(nne, cuda, d, t):
+    """Outputs of more than the L2s hold."""
+    rng = np.random.default_rng(70)
+    b, hq, hkv = 3, 32, 1
+    assert b * t * (hq + hkv) * d * 4 > 1 << 25
+    x = [rng.standard_normal((b, t, h, d), dtype=np.float32) for h in (hq, hkv)]
+    w = [1 + rng.standard_normal(d, dtype=np.float32) / 8 for _ in range(2)]
+    rope = nne.RotaryEmbedding(d, 4096, device=cuda)
+    start = np.array([0, 2000, 7], np.int32)
+    got = nne.qk_norm_rope(*(_up(a, cuda).transpose(1, 2) for a in x), *(_up(a, cuda) for a in w), rope,
+                           _up(start, cuda), start)
+    cos, sin = rope.cos.cpu().numpy(), rope.sin.cpu().numpy()
+    pos = start[:, None] + np.arange(t)
+    for g, src, weight in zip(got, x, w):
+        src = src.transpose(0, 2, 1, 3)
+        _close(g.cpu().numpy(), P.norm_rope64(src, weight, 1e-6, cos, sin, pos),
+               _norm_bound(src, weight, cos, sin, pos), "long")
+
+
 @pytest.mark.parametrize("norm", [False, True])
 @pytest.mark.parametrize("kind", ["token", "chain", "tree"])
 def test_layer_step(nne, cuda, norm, kind):
