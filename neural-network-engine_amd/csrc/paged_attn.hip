@@ -739,10 +739,13 @@ hipError_t launch_tile(const PagedAttnParams& p, hipStream_t stream) {
 
 template <bool BF16, int D>
 hipError_t launch_dim(const PagedAttnParams& p, hipStream_t stream) {
-    // (one row block: each byte of K and V is read by one workgroup)
-    if (p.tile_rows == 32) return launch_tile<BF16, D, 2, false, true>(p, stream);
-    if (p.T == 1 && p.n_rb == 1) return launch_tile<BF16, D, 1, true, false>(p, stream);
-    return launch_tile<BF16, D, 1, false, true>(p, stream);
+    // One row block: each byte of K and V is read by one workgroup, once (5 tokens of 16
+    // sequences of 512-4096 keys, bf16: 37 us, 43 through the caches).
+    const bool once = p.n_rb == 1;
+    if (p.tile_rows == 32)
+        return once ? launch_tile<BF16, D, 2, true, true>(p, stream) : launch_tile<BF16, D, 2, false, true>(p, stream);
+    if (p.T == 1 && once) return launch_tile<BF16, D, 1, true, false>(p, stream);
+    return once ? launch_tile<BF16, D, 1, true, true>(p, stream) : launch_tile<BF16, D, 1, false, true>(p, stream);
 }
 
 template <bool BF16>
