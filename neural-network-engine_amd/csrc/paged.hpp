@@ -58,9 +58,10 @@ struct PagedAttnParams {
     float* ws;                 // records: (max, sum) and O of rec_rows rows each
     uint32_t* cnt;             // arrivals per (sequence, KV head, row block)
     int combine;               // records are merged by a kernel of their own, not by the last to arrive
-    // Sequence b's keys are cut into prefix[b + 1] - prefix[b] equal parts, numbered
-    // through the launch.
+    // The keys of sequence b0 + order[i] are cut into prefix[i + 1] - prefix[i] equal
+    // parts, numbered through the launch.
     uint16_t prefix[kPagedSeqs + 1];
+    uint8_t order[kPagedSeqs];
 };
 
 // Dims of the tile.

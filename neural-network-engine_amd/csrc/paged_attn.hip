@@ -181,8 +181,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attent
     // Everything up to the first K and V is latency: one trip for the arguments,
     // one for the length, the page table and Q together, one for K and V.
     const int pref_lo = p.prefix[min(lane + 1, kPagedSeqs)], pref_hi = p.prefix[min(lane + 65, kPagedSeqs)];
+    const int order_lo = p.order[lane], order_hi = p.order[lane + 64];
     warm_kernargs<0, sizeof(PagedAttnParams)>();
-    asm volatile("" ::"v"(pref_lo), "v"(pref_hi));
+    asm volatile("" ::"v"(pref_lo), "v"(pref_hi), "v"(order_lo), "v"(order_hi));
     const PagedPool& pool = p.pool;
 
     // Workgroup -> (part of a sequence and KV head, row block).  With several row
@@ -196,9 +197,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attent
     }
     if (unit >= p.prefix[p.B] * pool.Hkv) return;
     const int part_all = quotient(unit, p.by_hkv), h = unit - part_all * pool.Hkv;
-    const int bl = __popcll(__builtin_amdgcn_ballot_w64(lane < p.B && pref_lo <= part_all)) +
-                   __popcll(__builtin_amdgcn_ballot_w64(lane + 64 < p.B && pref_hi <= part_all));
-    const int b = p.b0 + bl;
+    const int place = __popcll(__builtin_amdgcn_ballot_w64(lane < p.B && pref_lo <= part_all)) +
+                      __popcll(__builtin_amdgcn_ballot_w64(lane + 64 < p.B && pref_hi <= part_all));
+    const int b = p.b0 + __builtin_amdgcn_readlane(place < 64 ? order_lo : order_hi, place & 63);
     const int row0 = rb * ROWS;
     const int n_rows = min(ROWS, p.R - row0);
     const int raw_len = pool.lens[b];
@@ -259,8 +260,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attent
     // This part's keys, k0 to k1 of those that some row sees.
     const int len = paged_clamp(pool, raw_len);
     const int n_keys = block_keys(p, row0, n_rows, len, count);
-    const Parts parts = even_parts(p, p.prefix[bl], p.prefix[bl + 1] - p.prefix[bl], h, rb, n_keys, 4 * KB);
-    const int part = part_all - p.prefix[bl], live = parts.live;
+    const Parts parts = even_parts(p, p.prefix[place], p.prefix[place + 1] - p.prefix[place], h, rb, n_keys, 4 * KB);
+    const int part = part_all - p.prefix[place], live = parts.live;
     const int k0 = min(part * (int64_t)parts.length, (int64_t)n_keys);
     const int k1 = min((int64_t)n_keys, k0 + (int64_t)parts.length);
     if (k0 >= k1) return;
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attent
     // ---- the last of the parts to arrive merges their records in order
     wait_stores_performed();
     __syncthreads();
-    uint32_t* const cnt = p.cnt + ((int64_t)bl * pool.Hkv + h) * p.n_rb + rb;
+    uint32_t* const cnt = p.cnt + ((int64_t)place * pool.Hkv + h) * p.n_rb + rb;
     if (tid == 0)
         last_s = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)live - 1;
     __syncthreads();
@@ -679,11 +680,11 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnParam
         rb = unit - z * p.n_rb;
         unit = z;
     }
-    const int bl = quotient(unit, p.by_hkv), h = unit - bl * p.pool.Hkv, b = p.b0 + bl;
+    const int place = quotient(unit, p.by_hkv), h = unit - place * p.pool.Hkv, b = p.b0 + p.order[place];
     const int ROUND = p.pool.bf16 ? 128 : 64, row0 = rb * tile_rows, n_rows = min(tile_rows, p.R - row0);
     const int count = paged_count(p.counts, b, p.T), len = paged_len(p.pool, b);
     const int n_keys = block_keys(p, row0, n_rows, len, count);
-    const Parts parts = even_parts(p, p.prefix[bl], p.prefix[bl + 1] - p.prefix[bl], h, rb, n_keys, ROUND);
+    const Parts parts = even_parts(p, p.prefix[place], p.prefix[place + 1] - p.prefix[place], h, rb, n_keys, ROUND);
     const int f = blockIdx.y * 256 + threadIdx.x, rr = f / (D / 4), dd = 4 * (f % (D / 4));
     if (parts.live <= 1 || rr >= n_rows) return;
     const int64_t rec_floats = paged_record_floats(p.rec_rows, D), step = parts.rec_step * rec_floats;

@@ -2,6 +2,7 @@
 // share a sequence's rows and keys.
 #include <algorithm>
 #include <cmath>
+#include <functional>
 
 #include "paged.hpp"
 
@@ -33,6 +34,29 @@ float joined(float a, float b, float c) {
 
 // Upwards to a whole number (conversions, which vectorise where ceil is a call).
 float up(float x) { return (float)(int)(std::min(x, 1e9f) + .9999f); }
+
+// Fills p.order and p.prefix, sequence i in n_parts[i] parts.  Workgroups start in
+// this order: those with the longest parts first, so that the last to end are short
+// (32 sequences of 512-4096 keys, f32: 107.5 us, 109.9 as they come).  Where all run
+// at once, two on a CU, the second ones from the shortest on, so that each CU has a
+// long and a short one (256 rows of 8 sequences of 1024-4160 keys: 80 us, 86).
+void order_parts(PagedAttnParams& p, const int64_t* keys, const int64_t* n_parts, int64_t units, int cus) {
+    uint64_t by_length[kPagedSeqs];
+    int64_t total = 0, first = 0;
+    for (int i = 0; i < p.B; ++i) {
+        by_length[i] = (uint64_t)((keys[i] + n_parts[i] - 1) / n_parts[i]) << 8 | (uint64_t)(kPagedSeqs - 1 - i);
+        total += n_parts[i] * units;
+    }
+    std::sort(by_length, by_length + p.B, std::greater<uint64_t>());
+    for (int i = 0; i < p.B; ++i) p.order[i] = (uint8_t)(kPagedSeqs - 1 - (int)(by_length[i] & 255));
+    if (total > cus && total <= 2 * (int64_t)cus) {
+        int i = 0;
+        while (i < p.B && first < cus) first += n_parts[p.order[i++]] * units;
+        std::reverse(p.order + i, p.order + p.B);
+    }
+    p.prefix[0] = 0;
+    for (int i = 0; i < p.B; ++i) p.prefix[i + 1] = (uint16_t)(p.prefix[i] + n_parts[p.order[i]]);
+}
 
 }  // namespace
 
@@ -101,16 +125,13 @@ int64_t paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
     paged_set_tile(p, best_tile);
     const int64_t units = (int64_t)p.pool.Hkv * p.n_rb, best_len = (int64_t)best_rounds * step;
     const int64_t record = 4 * paged_record_floats(p.rec_rows, D);
-    int64_t parts = 0;
-    p.prefix[0] = 0;
-    for (int b = 0; b < p.B; ++b) {
-        parts += std::max<int64_t>(1, (keys[b] + best_len - 1) / best_len);
-        p.prefix[b + 1] = (uint16_t)parts;
-    }
+    int64_t n_parts[kPagedSeqs], parts = 0;
+    for (int b = 0; b < p.B; ++b) parts += n_parts[b] = std::max<int64_t>(1, (keys[b] + best_len - 1) / best_len);
     if (parts > p.B && (parts > UINT16_MAX || parts * units * record > most_bytes)) {   // (a rounding of the model's)
         parts = p.B;
-        for (int b = 0; b < p.B; ++b) p.prefix[b + 1] = (uint16_t)(b + 1);
+        std::fill(n_parts, n_parts + p.B, 1);
     }
+    order_parts(p, keys, n_parts, units, cus);
     p.combine = parts > p.B ? best_combine : 0;
     return parts > p.B ? parts * units : 0;
 }
