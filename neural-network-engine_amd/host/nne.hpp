@@ -304,6 +304,95 @@ class RotaryEmbedding {
     size_t head_dim, max_seq_len;
 };
 
+// The tokens of one step for each of a batch's sequences, as a tree (nne_attn.h,
+// "paged KV cache and drafted tokens"; no counterpart in the reference).
+class DraftTree {
+  public:
+    // parents [batch * tokens]: the token of its sequence that each one follows (an
+    // earlier one), or -1 for the last counted row.  counts [batch]: how many tokens of
+    // each sequence exist (empty: all).  Both go to the device once, here.  Throws
+    // std::invalid_argument for other values.
+    DraftTree(size_t batch, size_t tokens, std::vector<int32_t> parents, std::vector<int32_t> counts = {});
+    // Each token follows the one before.
+    static DraftTree chain(size_t batch, size_t tokens, std::vector<int32_t> counts = {});
+
+    size_t batch, tokens;
+    std::vector<int32_t> parents, depths, counts;        // host copies (empty: a chain, all tokens)
+    std::shared_ptr<int32_t> parents_dev, depths_dev, counts_dev;
+
+  private:
+    DraftTree() = default;
+    void set_counts(std::vector<int32_t> counts);
+};
+
+// A KV cache of pages shared by many sequences (nne_attn.h; the reference's caches are
+// a tensor per layer).  A step is, in each layer, append and attend; then one commit,
+// which accepts new rows: the first counts[b], or those of a tree's path.
+class PagedKVCache {
+  public:
+    enum class Dtype { F32 = NNE_F32, Bf16 = NNE_BF16 };
+    // Throws std::invalid_argument for a geometry that nne_attn.h does not take.
+    PagedKVCache(size_t num_layers, size_t num_pages, size_t num_kv_heads, size_t page_size, size_t head_dim,
+                 size_t batch, size_t max_pages_per_seq, Dtype dtype = Dtype::F32);
+
+    // Every sequence's pages, [batch * max_pages], -1 for none.
+    Result<bool> set_table(const std::vector<int32_t>& table);
+    // Declares rows [0, lens[b]) of each sequence filled.
+    Result<bool> set_lengths(const std::vector<int32_t>& lens);
+    // Pages for rows[b] rows of each sequence, out of those that none has; pages it has
+    // stay.  An error changes nothing.
+    Result<bool> allocate(const std::vector<size_t>& rows);
+    // Ends a sequence: no rows, no pages.
+    Result<bool> release(size_t seq);
+
+    // Rows of new tokens, k_new / v_new [B, Hkv, T, d], behind the counted ones, the
+    // keys rotated at their tokens' positions where rope is given.
+    Result<bool> append(size_t layer_idx, const RawTensor& k_new, const RawTensor& v_new,
+                        const RotaryEmbedding* rope = nullptr, const DraftTree* draft = nullptr);
+    // Their queries q [B, Hq, T, d] over the counted rows and those new ones that lead
+    // to them (zeros for tokens past a draft's counts).
+    Result<RawTensor> attend(size_t layer_idx, const RawTensor& q, const DraftTree* draft = nullptr,
+                             std::optional<float> scale = std::nullopt);
+    // Accepts the first counts[b] new rows of each sequence, or with paths [B * J] those
+    // of the tokens paths[b * J ..] (ascending), in every layer.
+    Result<bool> commit(const std::vector<int32_t>& counts, const std::vector<int32_t>& paths = {});
+
+    size_t num_layers() const { return num_layers_; }
+    size_t capacity() const { return max_pages * page_size; }
+    const std::vector<int32_t>& lengths() const { return lens_; }
+    const int32_t* lengths_device() const { return lens_dev_.get(); }
+    const std::vector<int32_t>& table() const { return table_; }
+    void* k_data(size_t layer_idx) const;                // [pages, Hkv, page_size, d]
+    void* v_data(size_t layer_idx) const;
+
+    size_t num_pages, num_kv_heads, page_size, head_dim, batch, max_pages;
+    Dtype dtype;
+
+  private:
+    Result<bool> check_layer(size_t layer_idx) const;
+    Result<bool> check_pages(const std::vector<int32_t>& table, const std::vector<int32_t>& lens) const;
+    Result<bool> check_draft(const DraftTree* draft, size_t tokens) const;
+    ::nne_paged_cache_t layer(size_t layer_idx) const;
+    const ::nne_workspace_t* workspace(const ::nne_paged_cache_t& c, size_t num_heads, size_t tokens);
+
+    size_t num_layers_;
+    std::shared_ptr<char> k_, v_;
+    std::vector<int32_t> table_, lens_;
+    std::shared_ptr<int32_t> table_dev_, lens_dev_, commit_dev_;
+    size_t commit_ints_ = 0;
+    std::shared_ptr<void> ws_;
+    std::shared_ptr<uint32_t> counters_;
+    std::shared_ptr<::nne_workspace_t> ws_desc_;
+};
+
+// Norm of every head of q and k [B, H, T, d] and rotation in one pass
+// (nne_qk_norm_rope), at the positions of a step over `cache`: new contiguous tensors.
+// Weights [d] or null (ones); eps null: no norm; rope null: no rotation.
+Result<std::pair<RawTensor, RawTensor>> qk_norm_rope(const RawTensor& q, const RawTensor& k, const RawTensor* q_weight,
+                                                     const RawTensor* k_weight, std::optional<float> eps,
+                                                     const RotaryEmbedding* rope, const PagedKVCache& cache,
+                                                     const DraftTree* draft = nullptr);
+
 // src/models/llama.rs:160-300, forward only.  Decode steps (t = 1 with a cache)
 // run the fused projection + RoPE launch on weights packed at construction and
 // the append + attend launch; other inputs project with GEMMs, rotate, append
@@ -326,12 +415,22 @@ class GroupedQueryAttention {
     Result<RawTensor> forward_gqa(const RawTensor& x, size_t start_pos) {   // :298-301
         return forward_gqa_cached(x, start_pos, nullptr);
     }
+    // A step over a paged cache: x [B, T, C] holds T new tokens of every sequence (a
+    // chain, or a DraftTree's), whose rows are appended and not yet counted: the caller
+    // commits once, after the last layer.
+    Result<RawTensor> forward_gqa_paged(const RawTensor& x, PagedKVCache& cache, size_t layer_idx = 0,
+                                        const DraftTree* draft = nullptr);
+    // Norms the heads of q and k before the rotation (weights [d]); taken by
+    // forward_gqa_paged alone.
+    void set_qk_norm(RawTensor q_weight, RawTensor k_weight, float eps = 1e-6f);
     // Re-packs q/k/v_proj weights for the fused decode projection; call after
     // changing them.
     void repack();
 
     Linear q_proj, k_proj, v_proj, o_proj;
     RotaryEmbedding rope;
+    std::optional<std::pair<RawTensor, RawTensor>> qk_norm;
+    float qk_norm_eps = 1e-6f;
     size_t num_heads, num_kv_heads, head_dim, num_queries_per_kv;
 
   private:

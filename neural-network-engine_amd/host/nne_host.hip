@@ -857,6 +857,335 @@ Result<RawTensor> GroupedQueryAttention::forward_gqa_cached(const RawTensor& x, 
     return forward_gqa_cached(x, start_pos, &layer_cache->cache(), layer_cache->layer_idx());
 }
 
+// ---- paged KV cache -----------------------------------------------------------------
+
+namespace {
+
+std::shared_ptr<int32_t> to_device(const std::vector<int32_t>& x) {
+    auto p = device_alloc<int32_t>(x.size());
+    if (!x.empty() && nne_memcpy_h2d(p.get(), x.data(), x.size() * 4, nullptr) != NNE_OK)
+        throw std::runtime_error(from_status(NNE_EHIP).to_string());
+    return p;
+}
+
+const int32_t* host_ptr(const std::vector<int32_t>& x) { return x.empty() ? nullptr : x.data(); }
+
+}  // namespace
+
+void DraftTree::set_counts(std::vector<int32_t> given) {
+    if (given.empty()) return;
+    if (given.size() != batch) throw std::invalid_argument("a draft's counts must be one per sequence");
+    for (int32_t n : given)
+        if (n < 0 || (size_t)n > tokens)
+            throw std::invalid_argument("counts outside [0, " + std::to_string(tokens) + "]");
+    counts = std::move(given);
+    counts_dev = to_device(counts);
+}
+
+DraftTree::DraftTree(size_t batch_, size_t tokens_, std::vector<int32_t> parents_, std::vector<int32_t> counts_)
+    : batch(batch_), tokens(tokens_), parents(std::move(parents_)) {
+    if (parents.size() != batch * tokens) throw std::invalid_argument("a draft's parents must be one per token");
+    depths.assign(parents.size(), 0);
+    for (size_t b = 0; b < batch; ++b) {
+        const size_t n = b < counts_.size() ? (size_t)std::max(counts_[b], 0) : tokens;
+        for (size_t t = 0; t < tokens; ++t) {
+            int32_t& p = parents[b * tokens + t];
+            if (t >= n) p = -1;                              // (does not exist)
+            if (p < -1 || p >= (int32_t)t)
+                throw std::invalid_argument("a token's parent comes before it (-1: the sequence's last row)");
+            if (p >= 0) depths[b * tokens + t] = depths[b * tokens + p] + 1;
+        }
+    }
+    set_counts(std::move(counts_));
+    parents_dev = to_device(parents);
+    depths_dev = to_device(depths);
+}
+
+DraftTree DraftTree::chain(size_t batch, size_t tokens, std::vector<int32_t> counts) {
+    DraftTree d;
+    d.batch = batch;
+    d.tokens = tokens;
+    d.set_counts(std::move(counts));
+    return d;
+}
+
+PagedKVCache::PagedKVCache(size_t num_layers, size_t num_pages_, size_t num_kv_heads_, size_t page_size_,
+                           size_t head_dim_, size_t batch_, size_t max_pages_per_seq, Dtype dtype_)
+    : num_pages(num_pages_), num_kv_heads(num_kv_heads_), page_size(page_size_), head_dim(head_dim_), batch(batch_),
+      max_pages(max_pages_per_seq), dtype(dtype_), num_layers_(num_layers) {
+    // The C ABI's checks of the geometry, before anything is allocated.
+    static int32_t none;
+    const nne_paged_cache_t c{nullptr, nullptr, (int64_t)dtype, (int64_t)num_pages, (int64_t)num_kv_heads,
+                              (int64_t)page_size, (int64_t)head_dim, (int64_t)batch, (int64_t)max_pages,
+                              nullptr, nullptr, nullptr, &none};
+    nne_workspace_size_t need;
+    if (nne_paged_workspace_size(&c, (int64_t)num_kv_heads, 0, &need) != NNE_OK)
+        throw std::invalid_argument(from_status(NNE_EINVAL).message);
+    const size_t bytes = num_layers * num_pages * num_kv_heads * page_size * head_dim * (dtype == Dtype::F32 ? 4 : 2);
+    k_ = device_alloc<char>(bytes);
+    v_ = device_alloc<char>(bytes);
+    if (bytes) {
+        hip_check(hipMemset(k_.get(), 0, bytes), "hipMemset");
+        hip_check(hipMemset(v_.get(), 0, bytes), "hipMemset");
+    }
+    table_.assign(batch * max_pages, -1);
+    lens_.assign(batch, 0);
+    table_dev_ = to_device(table_);
+    lens_dev_ = to_device(lens_);
+}
+
+void* PagedKVCache::k_data(size_t i) const {
+    return k_.get() + i * num_pages * num_kv_heads * page_size * head_dim * (dtype == Dtype::F32 ? 4 : 2);
+}
+
+void* PagedKVCache::v_data(size_t i) const {
+    return v_.get() + i * num_pages * num_kv_heads * page_size * head_dim * (dtype == Dtype::F32 ? 4 : 2);
+}
+
+nne_paged_cache_t PagedKVCache::layer(size_t i) const {
+    return nne_paged_cache_t{k_data(i), v_data(i), (int64_t)dtype, (int64_t)num_pages, (int64_t)num_kv_heads,
+                             (int64_t)page_size, (int64_t)head_dim, (int64_t)batch, (int64_t)max_pages,
+                             table_dev_.get(), table_.data(), lens_dev_.get(), const_cast<int32_t*>(lens_.data())};
+}
+
+Result<bool> PagedKVCache::check_layer(size_t layer_idx) const {
+    if (layer_idx >= num_layers_)
+        return EngineError::invalid_argument("PagedKVCache layer index " + std::to_string(layer_idx) +
+                                             " out of range (total layers: " + std::to_string(num_layers_) + ")");
+    return true;
+}
+
+Result<bool> PagedKVCache::check_pages(const std::vector<int32_t>& table, const std::vector<int32_t>& lens) const {
+    for (int32_t p : table)
+        if (p < -1 || p >= (int64_t)num_pages)
+            return EngineError::invalid_argument("page " + std::to_string(p) + " outside [0, " +
+                                                 std::to_string(num_pages) + ")");
+    for (size_t b = 0; b < batch; ++b)
+        for (size_t i = 0; i < ((size_t)lens[b] + page_size - 1) / page_size; ++i)
+            if (table[b * max_pages + i] < 0) return EngineError::invalid_argument("a counted row has no page");
+    return true;
+}
+
+Result<bool> PagedKVCache::check_draft(const DraftTree* draft, size_t tokens) const {
+    if (draft && (draft->batch != batch || draft->tokens != tokens))
+        return EngineError::shape_mismatch({draft->batch, draft->tokens}, {batch, tokens});
+    return true;
+}
+
+Result<bool> PagedKVCache::set_table(const std::vector<int32_t>& table) {
+    if (table.size() != table_.size()) return EngineError::shape_mismatch({batch, max_pages}, {table.size()});
+    auto ok = check_pages(table, lens_);
+    if (ok.is_err()) return ok;
+    table_ = table;
+    if (!table_.empty() && nne_memcpy_h2d(table_dev_.get(), table_.data(), table_.size() * 4, nullptr) != NNE_OK)
+        return from_status(NNE_EHIP);
+    return true;
+}
+
+Result<bool> PagedKVCache::set_lengths(const std::vector<int32_t>& lens) {
+    if (lens.size() != batch) return EngineError::shape_mismatch({batch}, {lens.size()});
+    for (int32_t n : lens)
+        if (n < 0 || (size_t)n > capacity())
+            return EngineError::invalid_argument("sequence length " + std::to_string(n) + " outside [0, " +
+                                                 std::to_string(capacity()) + "]");
+    auto ok = check_pages(table_, lens);
+    if (ok.is_err()) return ok;
+    std::copy(lens.begin(), lens.end(), lens_.begin());
+    if (batch && nne_memcpy_h2d(lens_dev_.get(), lens_.data(), batch * 4, nullptr) != NNE_OK)
+        return from_status(NNE_EHIP);
+    return true;
+}
+
+Result<bool> PagedKVCache::allocate(const std::vector<size_t>& rows) {
+    if (rows.size() != batch) return EngineError::shape_mismatch({batch}, {rows.size()});
+    std::vector<char> used(num_pages, 0);
+    for (int32_t p : table_)
+        if (p >= 0) used[p] = 1;
+    std::vector<int32_t> table = table_;
+    size_t next = 0;
+    for (size_t b = 0; b < batch; ++b) {
+        if (rows[b] > capacity())
+            return EngineError::gpu_error(std::to_string(rows[b]) + " rows exceed " + std::to_string(max_pages) +
+                                          " pages of " + std::to_string(page_size) + " rows");
+        for (size_t i = 0; i < (rows[b] + page_size - 1) / page_size; ++i) {
+            int32_t& p = table[b * max_pages + i];
+            if (p >= 0) continue;
+            while (next < num_pages && used[next]) ++next;
+            if (next == num_pages)
+                return EngineError::gpu_error("no page of " + std::to_string(num_pages) + " is free");
+            p = (int32_t)next++;
+        }
+    }
+    return set_table(table);
+}
+
+Result<bool> PagedKVCache::release(size_t seq) {
+    if (seq >= batch)
+        return EngineError::invalid_argument("sequence " + std::to_string(seq) + " of " + std::to_string(batch));
+    std::vector<int32_t> lens = lens_, table = table_;
+    lens[seq] = 0;
+    std::fill(table.begin() + seq * max_pages, table.begin() + (seq + 1) * max_pages, -1);
+    auto ok = set_lengths(lens);
+    if (ok.is_err()) return ok;
+    return set_table(table);
+}
+
+Result<bool> PagedKVCache::append(size_t layer_idx, const RawTensor& k_new, const RawTensor& v_new,
+                                  const RotaryEmbedding* rope, const DraftTree* draft) {
+    auto ok = check_layer(layer_idx);
+    if (ok.is_err()) return ok;
+    const size_t t = k_new.ndim() == 4 ? k_new.shape()[2] : 0;
+    const std::vector<size_t> want{batch, num_kv_heads, t, head_dim};
+    if (k_new.shape() != want) return EngineError::shape_mismatch(want, k_new.shape());
+    if (v_new.shape() != want) return EngineError::shape_mismatch(want, v_new.shape());
+    ok = check_draft(draft, t);
+    if (ok.is_err()) return ok;
+    if (rope && rope->head_dim != head_dim) return EngineError::shape_mismatch({rope->head_dim}, {head_dim});
+    const nne_paged_cache_t c = layer(layer_idx);
+    const auto kst = as_i64(k_new.strides()), vst = as_i64(v_new.strides());
+    const int rc = nne_paged_append(&c, k_new.data(), kst.data(), v_new.data(), vst.data(), (int64_t)t,
+                                    draft ? draft->counts_dev.get() : nullptr, draft ? host_ptr(draft->counts) : nullptr,
+                                    draft ? draft->depths_dev.get() : nullptr, draft ? host_ptr(draft->depths) : nullptr,
+                                    rope ? rope->cos_cached.data() : nullptr, rope ? rope->sin_cached.data() : nullptr,
+                                    rope ? (int64_t)rope->max_seq_len : 0, rope ? (int64_t)rope->head_dim : 0, nullptr);
+    if (rc != NNE_OK) return from_status(rc);
+    return true;
+}
+
+const nne_workspace_t* PagedKVCache::workspace(const nne_paged_cache_t& c, size_t num_heads, size_t tokens) {
+    nne_workspace_size_t need{0, (uint64_t)batch};
+    if (tokens && nne_paged_workspace_size(&c, (int64_t)num_heads, (int64_t)tokens, &need) != NNE_OK)
+        return nullptr;   // the call itself reports the geometry error
+    if (!ws_desc_) ws_desc_ = std::make_shared<nne_workspace_t>(nne_workspace_t{nullptr, 0, nullptr, 0});
+    nne_workspace_t& w = *ws_desc_;
+    if (need.records_bytes > w.records_bytes) {
+        auto buf = device_alloc<char>(need.records_bytes);
+        ws_ = std::shared_ptr<void>(buf, buf.get());
+        w.records = ws_.get();
+        w.records_bytes = need.records_bytes;
+    }
+    if (need.n_counters > w.n_counters) {
+        counters_ = device_alloc<uint32_t>(need.n_counters);
+        if (nne_counters_init(counters_.get(), need.n_counters, nullptr) != NNE_OK)
+            throw std::runtime_error(from_status(NNE_EHIP).to_string());
+        w.counters = counters_.get();
+        w.n_counters = need.n_counters;
+    }
+    return ws_desc_.get();
+}
+
+Result<RawTensor> PagedKVCache::attend(size_t layer_idx, const RawTensor& q, const DraftTree* draft,
+                                       std::optional<float> scale) {
+    auto ok = check_layer(layer_idx);
+    if (ok.is_err()) return ok.error();
+    if (q.ndim() != 4 || q.shape()[0] != batch || q.shape()[3] != head_dim)
+        return EngineError::shape_mismatch({batch, q.ndim() == 4 ? q.shape()[1] : 0, q.ndim() == 4 ? q.shape()[2] : 0,
+                                            head_dim}, q.shape());
+    const size_t hq = q.shape()[1], t = q.shape()[2];
+    ok = check_draft(draft, t);
+    if (ok.is_err()) return ok.error();
+    const nne_paged_cache_t c = layer(layer_idx);
+    RawTensor out = RawTensor::zeros(q.shape());
+    const auto qst = as_i64(q.strides()), ost = as_i64(out.strides());
+    const int rc = nne_paged_attention(
+        &c, q.data(), qst.data(), out.data(), ost.data(), (int64_t)hq, (int64_t)t,
+        draft ? draft->counts_dev.get() : nullptr, draft ? host_ptr(draft->counts) : nullptr,
+        draft ? draft->parents_dev.get() : nullptr, draft ? host_ptr(draft->parents) : nullptr, scale ? 1 : 0,
+        scale.value_or(0.f), workspace(c, hq, t), nullptr);
+    if (rc != NNE_OK) return from_status(rc);
+    return out;
+}
+
+Result<bool> PagedKVCache::commit(const std::vector<int32_t>& counts, const std::vector<int32_t>& paths) {
+    if (num_layers_ == 0) return EngineError::invalid_argument("a cache of no layers");
+    if (counts.size() != batch) return EngineError::shape_mismatch({batch}, {counts.size()});
+    if (batch && paths.size() % batch != 0) return EngineError::shape_mismatch({batch, 0}, {paths.size()});
+    if (batch == 0) return true;
+    size_t j = paths.size() / batch;
+    if (paths.empty()) j = (size_t)std::max(*std::max_element(counts.begin(), counts.end()), 0);
+    const size_t ints = batch + paths.size();
+    if (ints > commit_ints_) {
+        commit_dev_ = device_alloc<int32_t>(ints);
+        commit_ints_ = ints;
+    }
+    int32_t* const dev = commit_dev_.get();
+    if (nne_memcpy_h2d(dev, counts.data(), batch * 4, nullptr) != NNE_OK ||
+        (!paths.empty() && nne_memcpy_h2d(dev + batch, paths.data(), paths.size() * 4, nullptr) != NNE_OK))
+        return from_status(NNE_EHIP);
+    const nne_paged_cache_t c = layer(0);
+    const int rc = nne_paged_commit(&c, (int64_t)num_layers_, (int64_t)(num_pages * num_kv_heads * page_size * head_dim),
+                                    dev, counts.data(), paths.empty() ? nullptr : dev + batch, host_ptr(paths),
+                                    (int64_t)j, workspace(c, num_kv_heads, 0), nullptr);
+    if (rc != NNE_OK) return from_status(rc);
+    return true;
+}
+
+Result<std::pair<RawTensor, RawTensor>> qk_norm_rope(const RawTensor& q, const RawTensor& k, const RawTensor* q_weight,
+                                                     const RawTensor* k_weight, std::optional<float> eps,
+                                                     const RotaryEmbedding* rope, const PagedKVCache& cache,
+                                                     const DraftTree* draft) {
+    if (q.ndim() != 4 || k.ndim() != 4)
+        return EngineError::incompatible_shapes("qk_norm_rope (expected 4D inputs [B, H, T, d])", {q.shape(), k.shape()});
+    const size_t b = q.shape()[0], t = q.shape()[2], d = q.shape()[3];
+    const std::vector<size_t> want{b, k.shape()[1], t, d};
+    if (k.shape() != want) return EngineError::shape_mismatch(want, k.shape());
+    if (b != cache.batch) return EngineError::shape_mismatch({cache.batch}, {b});
+    if (draft && (draft->batch != b || draft->tokens != t))
+        return EngineError::shape_mismatch({draft->batch, draft->tokens}, {b, t});
+    if (rope && rope->head_dim != d) return EngineError::shape_mismatch({rope->head_dim}, {d});
+    for (const RawTensor* w : {q_weight, k_weight})
+        if (w && (w->ndim() != 1 || w->shape()[0] != d || !w->is_contiguous()))
+            return EngineError::shape_mismatch({d}, w->shape());
+    RawTensor qo = RawTensor::zeros(q.shape()), ko = RawTensor::zeros(k.shape());
+    const auto qs = as_i64(q.shape()), qst = as_i64(q.strides()), qot = as_i64(qo.strides());
+    const auto ks = as_i64(k.shape()), kst = as_i64(k.strides()), kot = as_i64(ko.strides());
+    const int rc = nne_qk_norm_rope(
+        q.data(), qs.data(), qst.data(), qo.data(), qot.data(), k.data(), ks.data(), kst.data(), ko.data(), kot.data(),
+        q_weight ? q_weight->data() : nullptr, k_weight ? k_weight->data() : nullptr, eps ? 1 : 0, eps.value_or(0.f),
+        rope ? rope->cos_cached.data() : nullptr, rope ? rope->sin_cached.data() : nullptr,
+        rope ? (int64_t)rope->max_seq_len : 0, rope ? (int64_t)rope->head_dim : 0, cache.lengths_device(),
+        cache.lengths().data(), draft ? draft->depths_dev.get() : nullptr, draft ? host_ptr(draft->depths) : nullptr,
+        nullptr);
+    if (rc != NNE_OK) return from_status(rc);
+    return std::make_pair(qo, ko);
+}
+
+void GroupedQueryAttention::set_qk_norm(RawTensor q_weight, RawTensor k_weight, float eps) {
+    qk_norm = std::make_pair(std::move(q_weight), std::move(k_weight));
+    qk_norm_eps = eps;
+}
+
+Result<RawTensor> GroupedQueryAttention::forward_gqa_paged(const RawTensor& x, PagedKVCache& cache, size_t layer_idx,
+                                                           const DraftTree* draft) {
+    if (x.ndim() != 3)
+        return EngineError::incompatible_shapes("GroupedQueryAttention forward (expected 3D input [B, T, C])",
+                                                {x.shape()});
+    const size_t b = x.shape()[0], t = x.shape()[1], c = x.shape()[2], d = head_dim;
+    if (c != q_proj.in_features)
+        return EngineError::incompatible_shapes("matmul_transposed_b", {x.shape(), q_proj.weight.shape()});
+    if (cache.batch != b || cache.num_kv_heads != num_kv_heads || cache.head_dim != d)
+        return EngineError::shape_mismatch({b, num_kv_heads, d}, {cache.batch, cache.num_kv_heads, cache.head_dim});
+    auto qp = q_proj.forward(x);
+    if (qp.is_err()) return qp.error();
+    auto kp = k_proj.forward(x);
+    if (kp.is_err()) return kp.error();
+    auto vp = v_proj.forward(x);
+    if (vp.is_err()) return vp.error();
+    auto heads = [&](const RawTensor& y, size_t h) {
+        return y.reshape({b, t, h, d}).value().transpose(1, 2).value();
+    };
+    auto qk = qk_norm_rope(heads(qp.value(), num_heads), heads(kp.value(), num_kv_heads),
+                           qk_norm ? &qk_norm->first : nullptr, qk_norm ? &qk_norm->second : nullptr,
+                           qk_norm ? std::optional<float>(qk_norm_eps) : std::nullopt, &rope, cache, draft);
+    if (qk.is_err()) return qk.error();
+    auto ok = cache.append(layer_idx, qk.value().second, heads(vp.value(), num_kv_heads), nullptr, draft);
+    if (ok.is_err()) return ok.error();
+    auto ctx = cache.attend(layer_idx, qk.value().first, draft);
+    if (ctx.is_err()) return ctx.error();
+    RawTensor merged = ctx.value().transpose(1, 2).value().to_contiguous();
+    return o_proj.forward(merged.reshape({b, t, num_heads * d}).value());
+}
+
 // ---- MultiHeadAttention -----------------------------------------------------------
 
 MultiHeadAttention::MultiHeadAttention(size_t d_model_, size_t num_heads_, bool is_causal_)
