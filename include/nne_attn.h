@@ -427,7 +427,8 @@ int nne_paged_append(const nne_paged_cache_t *cache, const float *k_new,
  * the lens[b] counted rows, and of the new ones itself and those before it on
  * its path.  Rows of o for tokens past counts[b] are left as they were.  At
  * most 256 tokens with parents, any number in a chain.  What a token does not
- * see has no part in its result, whatever it holds.  ws: at least
+ * see has no part in its result, whatever it holds; an infinite or NaN value that
+ * it sees makes the result infinite or NaN.  ws: at least
  * nne_paged_workspace_size, or NULL for the library's per-stream one (a stream
  * under capture must have one that is large enough already: NNE_EINVAL). */
 int nne_paged_attention(const nne_paged_cache_t *cache, const float *q, const int64_t q_strides[4],

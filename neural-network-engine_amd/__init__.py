@@ -797,6 +797,8 @@ def _new_like(t, stream):
 
 
 def _int_array(x, shape, what):
+    if x is None:
+        raise InvalidArgument("Invalid configuration or argument: %s is missing" % what)
     a = x
     if type(a) is not np.ndarray or a.dtype != np.int32 or not a.flags.c_contiguous:
         a = np.ascontiguousarray(x, dtype=np.int32)
@@ -807,7 +809,7 @@ def _int_array(x, shape, what):
 
 
 def _check_int_dev(t, shape, index, what):
-    if t.dtype is not _torch.int32 or t.get_device() != index or t.shape != shape or \
+    if t is None or t.dtype is not _torch.int32 or t.get_device() != index or t.shape != shape or \
             not t.is_contiguous():
         raise InvalidArgument("Invalid configuration or argument: %s must be a contiguous int32 "
                               "tensor of shape %s on GPU %d" % (what, list(shape), index))
@@ -1000,7 +1002,12 @@ class PagedKVCache:
     A step of one or more new tokens per sequence is, in each layer, ``append``
     (their rows go behind the counted ones) and ``attend``; then once ``commit``,
     which accepts new rows: all, the first few, or the path of a ``DraftTree``.
-    Until then a further append writes the same rows again."""
+    Until then a further append writes the same rows again.
+
+    Calls on one cache go in the order of one stream: they share its lengths and its
+    workspace.  Tables and lengths are set on the current stream.  A captured step
+    needs ``reserve_workspace`` (or an eager step of its size) before, and after its
+    replays ``set_lengths`` tells the host what the device has counted."""
 
     def __init__(self, num_layers, num_pages, num_kv_heads, page_size, head_dim, batch,
                  max_pages_per_seq, dtype=None, device="cuda"):
@@ -1021,14 +1028,31 @@ class PagedKVCache:
         self._v = torch.zeros(shape, dtype=self.dtype, device=device)
         self._device = self._k.device
         self._index = self._k.get_device()
-        self.table_host = np.full((self.batch, self.max_pages), -1, np.int32)
-        self.table_dev = torch.full((self.batch, self.max_pages), -1, dtype=torch.int32,
+        self._table_host = np.full((self.batch, self.max_pages), -1, np.int32)
+        self._table_dev = torch.full((self.batch, self.max_pages), -1, dtype=torch.int32,
                                     device=device)
-        self.lens_host = np.zeros(self.batch, np.int32)
-        self.lens_dev = torch.zeros(self.batch, dtype=torch.int32, device=device)
+        self._lens_host = np.zeros(self.batch, np.int32)
+        self._lens_dev = torch.zeros(self.batch, dtype=torch.int32, device=device)
         self._ws = _StepWorkspace(self._device)
         self._sizes, self._ws_ready = {}, {}
         self._bind()
+
+    # The calls hold on to these arrays: their values change, they do not.
+    @property
+    def table_host(self):
+        return self._table_host
+
+    @property
+    def table_dev(self):
+        return self._table_dev
+
+    @property
+    def lens_host(self):
+        return self._lens_host
+
+    @property
+    def lens_dev(self):
+        return self._lens_dev
 
     @property
     def k(self):
@@ -1069,10 +1093,10 @@ class PagedKVCache:
         def struct(i, table_host):
             return NnePagedCache(k + i * step, v + i * step, int(size == 2), self.num_pages,
                                  self.num_kv_heads, self.page_size, self.head_dim, self.batch,
-                                 self.max_pages, self.table_dev.data_ptr(), table_host,
-                                 self.lens_dev.data_ptr(), self.lens_host.ctypes.data)
+                                 self.max_pages, self._table_dev.data_ptr(), table_host,
+                                 self._lens_dev.data_ptr(), self._lens_host.ctypes.data)
 
-        host = self.table_host.ctypes.data
+        host = self._table_host.ctypes.data
         self._structs = [(struct(i, host), struct(i, None)) for i in range(self._shape[0])]
         self._addr = [tuple(ctypes.addressof(s) for s in pair) for pair in self._structs]
 
@@ -1106,11 +1130,11 @@ class PagedKVCache:
         if table.ndim != 2 or table.shape[0] != self.batch or table.shape[1] > self.max_pages:
             raise ShapeMismatch("Shape mismatch error: expected shape %s, got %s"
                                 % ([self.batch, self.max_pages], list(table.shape)))
-        full = np.full_like(self.table_host, -1)
+        full = np.full_like(self._table_host, -1)
         full[:, :table.shape[1]] = table
-        self._check_pages(full, self.lens_host)
-        self.table_host[...] = full
-        self.table_dev.copy_(torch.from_numpy(full))
+        self._check_pages(full, self._lens_host)
+        self._table_host[...] = full
+        self._table_dev.copy_(torch.from_numpy(full))
 
     def set_lengths(self, lens):
         """Declares that rows [0, lens[b]) of every sequence are filled."""
@@ -1118,9 +1142,9 @@ class PagedKVCache:
         lens = np.asarray(lens, dtype=np.int32)
         if lens.shape != (self.batch,) or (lens < 0).any() or (lens > self.capacity()).any():
             raise InvalidArgument("Invalid configuration or argument: bad lengths")
-        self._check_pages(self.table_host, lens)
-        self.lens_host[:] = lens
-        self.lens_dev.copy_(torch.from_numpy(lens.copy()))
+        self._check_pages(self._table_host, lens)
+        self._lens_host[:] = lens
+        self._lens_dev.copy_(torch.from_numpy(lens.copy()))
 
     def allocate(self, rows):
         """Gives every sequence pages for rows[b] rows (an int: the same for
@@ -1130,8 +1154,10 @@ class PagedKVCache:
         if (rows > self.capacity()).any():
             raise CapacityError("GPU compute error: %d rows exceed %d pages of %d rows"
                                 % (rows.max(), self.max_pages, self.page_size))
-        table = self.table_host.copy()
-        free = np.setdiff1d(np.arange(self.num_pages, dtype=np.int32), table)
+        table = self._table_host.copy()
+        free = np.ones(self.num_pages, bool)
+        free[table[table >= 0]] = False
+        free = np.flatnonzero(free)
         wanted = (np.arange(self.max_pages) < -(-rows // self.page_size)[:, None]) & (table < 0)
         if int(wanted.sum()) > len(free):
             raise CapacityError("GPU compute error: %d pages wanted, %d of %d are free"
@@ -1144,7 +1170,7 @@ class PagedKVCache:
         if not 0 <= seq < self.batch:
             raise InvalidArgument("Invalid configuration or argument: sequence %d of %d"
                                   % (seq, self.batch))
-        lens, table = self.lens_host.copy(), self.table_host.copy()
+        lens, table = self._lens_host.copy(), self._table_host.copy()
         lens[seq], table[seq] = 0, -1
         self.set_lengths(lens)
         self.set_table(table)

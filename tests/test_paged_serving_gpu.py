@@ -519,6 +519,10 @@ def test_python_calls_refuse(nne, cuda):
             (bad, lambda: nne.qk_norm_rope(q, None, None, None, None, None, None, k_out=x)),
             (bad, lambda: nne.qk_norm_rope(q, x, torch.ones(16, device=cuda), None, None, None, None, eps=None)),
             (bad, lambda: nne.qk_norm_rope(q, x.cpu(), None, None, None, None, None)),
+            (bad, lambda: nne.qk_norm_rope(q, x, None, None, nne.RotaryEmbedding(16, 64, device=cuda), None, None)),
+            (bad, lambda: nne.qk_norm_rope(q, x, None, None, nne.RotaryEmbedding(16, 64, device=cuda), None, [0, 0])),
+            (bad, lambda: cache.commit(torch.zeros(2, dtype=torch.int32, device=cuda))),
+            (AttributeError, lambda: setattr(cache, "lens_host", np.zeros(2, np.int32))),
     ]:
         with pytest.raises(error):
             call()
