@@ -318,6 +318,18 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attent
         return (u < 0) | (((anc_s[t][at >> 5] >> (at & 31)) & 1u) != 0);
     };
 
+    // The same for drafted tokens u0, u0 + 1, ..., a bit each.
+    auto sees_from = [&](int t, int u0) __attribute__((always_inline)) -> uint32_t {
+        if (!p.parents) {
+            const int n = t - u0 + 1;
+            return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u;
+        }
+        const int w = u0 >> 5;           // (uniform; u0 > -32)
+        const uint32_t lo = w < 0 ? ~0u : anc_s[t][min(w, kPagedTreeNodes / 32 - 1)];
+        const uint32_t hi = w + 1 < kPagedTreeNodes / 32 ? anc_s[t][w + 1] : 0u;
+        return __builtin_amdgcn_alignbit(hi, lo, (uint32_t)u0 & 31u);
+    };
+
     floatx4 o[NRT][NO];
     float m_run[NRT], l_run[NRT];
 #pragma unroll
@@ -428,22 +440,30 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : DRAFT ? 2 : 3) void paged_attent
             const bool drafted = DRAFT && p.T > 1 && kb + KB > len;
             const uint32_t gone = (uint32_t)__builtin_amdgcn_readfirstlane((int)gone_s[blk * KB >> 5]) >> (blk * KB & 31);
             if (__builtin_expect((gone << (32 - KB)) != 0 || drafted, 0)) {
+                // A word of bits per row tile, bit i for the block's key i, so that a
+                // lane's keys are at constant places from 4 g on.
                 int gm = g;              // (nothing of this is worth a register in the other blocks)
                 asm volatile("" : "+v"(gm));
+                const uint32_t there = ~gone >> (4 * gm);
+                uint32_t ok[NRT];
+#pragma unroll
+                for (int rt = 0; rt < NRT; ++rt) ok[rt] = there;
+                if (drafted)
+#pragma unroll
+                    for (int rt = 0; rt < NRT; ++rt) ok[rt] &= sees_from(tok[rt], kb - len) >> (4 * gm);
 #pragma unroll
                 for (int j = 0; j < JN; ++j) {
-                    const int in = slot_key<BF16>(gm, j);
-                    const bool there = ((gone >> in) & 1u) == 0;
+                    const int at = 31 - slot_key<BF16>(0, j);
 #pragma unroll
                     for (int rt = 0; rt < NRT; ++rt) {
-                        const bool ok = there & (!drafted | sees(tok[rt], kb + in - len));
-                        const float x = s[rt][j >> 2][j & 3];
-                        s[rt][j >> 2][j & 3] = ok ? x : kNegInf;
+                        const uint32_t m = (uint32_t)((int)(ok[rt] << at) >> 31), x = __float_as_uint(s[rt][j >> 2][j & 3]);
+                        s[rt][j >> 2][j & 3] = __uint_as_float((x & m) | (~m & 0xff800000u));     // (-infinity)
                     }
+                    const uint32_t m = (uint32_t)((int)(there << at) >> 31);
 #pragma unroll
                     for (int c = 0; c < NV; ++c)
 #pragma unroll
-                        for (int w = 0; w < (int)(sizeof(VReg) / 4); ++w) vreg[j][c][w] = there ? vreg[j][c][w] : 0u;
+                        for (int w = 0; w < (int)(sizeof(VReg) / 4); ++w) vreg[j][c][w] &= m;
                 }
             }
 
