@@ -12,18 +12,19 @@ namespace {
 
 constexpr int kTargetPerCu = 4;    // workgroups per CU that a split may make
 
-// Times of the kernel, fitted to 2200 launches of 60 shapes (1-62 sequences of 5-8000
-// keys, 1-256 rows, head dims 64-256, both types, parts of 128-8448 keys; rms error of
-// the fit 8 %; the part length it picks is 1.2 % above the best of those timed).
-// Rows: tiles of 16 and of 32 rows; columns: f32 and bf16 pools.
-constexpr float kStart[2][2] = {{0.f, 1.0f}, {0.6f, 4.4f}};         // us of a workgroup
-constexpr float kStartDims[2][2] = {{2.8f, 1.5f}, {3.8f, 1.7f}};    // and per 128 dims
-constexpr float kKey[2][2] = {{.0063f, .0051f}, {0.f, 0.f}};        // us of a key
-constexpr float kKeyDims[2][2] = {{.0148f, .0055f}, {.0325f, .0148f}};
-constexpr float kAtOnce[2][2] = {{1.14f, 1.08f}, {1.05f, 1.40f}};   // gain of several on a CU
-constexpr float kBytesPerUs = 5.76e6f;
-constexpr float kMerge = 0.8f, kMergePart = .072f, kMergeFloat = 1.04e-4f;   // by the last to arrive
-constexpr float kCombine = 3.7f, kCombinePart = .042f;                       // by a launch of its own
+// Times of the kernel, fitted to 2750 launches of 190 shapes (1-64 sequences of 5-8000
+// keys, 1-512 rows, both types, parts of 128-8448 keys; rms error of the fit 8 %; the
+// tile and part length it picks take 1.0 % more than the best of those timed).
+// [tiles of 16, of 32 rows][f32, bf16 pools][dims up to 64, 128, 256]
+constexpr float kStart[2][2][3] = {{{2.6f, 3.4f, 4.3f}, {3.2f, 3.1f, 4.7f}},       // us of a workgroup
+                                   {{3.7f, 5.5f, 9.2f}, {4.8f, 5.7f, 8.4f}}};
+constexpr float kKey[2][2][3] = {{{.0131f, .0195f, .0240f}, {.0073f, .0102f, .0146f}},   // us of a key
+                                 {{.0198f, .0312f, .0536f}, {.0080f, .0131f, .0172f}}};
+constexpr float kAtOnce[2][2][3] = {{{1.41f, 1.04f, .60f}, {1.83f, 1.19f, .78f}},  // gain of several on a CU
+                                    {{1.18f, 1.03f, .84f}, {1.74f, 1.38f, .81f}}};
+constexpr float kBytesPerUs = 5.77e6f;
+constexpr float kMerge = 1.74f, kMergePart = .080f, kMergeFloat = 7.6e-5f;   // by the last to arrive
+constexpr float kCombine = 4.3f, kCombinePart = .034f;                       // by a launch of its own
 
 // Sum of the fourth powers' root: the largest of the three, with the overlap of
 // those that come near it.
@@ -87,16 +88,15 @@ int64_t paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
     const float memory = sum * (float)(p.pool.Hkv * p.pool.d * (p.pool.bf16 ? 4 : 8)) / kBytesPerUs;
     // Tiles of 16 rows start sooner and spread few rows over more CUs, tiles of 32
     // bring K and V half as often: 52 rows of a sequence of 1746 keys take 16.3 and
-    // 18.6 us, 256 rows of 8 sequences of 1024-4160 keys 127 and 86.  The part length
+    // 18.6 us, 256 rows of 8 sequences of 1024-4160 keys 127 and 80.  The part length
     // and the tile of least modelled time: a workgroup pays a fixed time and its
     // keys, a CU its share of them, the memory the bytes, and parts pay their merge.
     int best_tile = 16, best_combine = 0;
     float best = 1e30f, best_rounds = longest;
     for (int tile = 16; tile <= (p.R > 16 ? 32 : 16); tile += 16) {
-        const int at = tile / 32, rows = std::min(p.R, tile);
-        const float units = (float)p.pool.Hkv * (float)((p.R + tile - 1) / tile);   // workgroups of a part
-        const float start = kStart[at][type] + kStartDims[at][type] * (float)D / 128.f;
-        const float key = kKey[at][type] + kKeyDims[at][type] * (float)D / 128.f;
+        const int at = tile / 32, dims = D / 128, rows = std::min(p.R, tile);
+        const float n_rb = (float)((p.R + tile - 1) / tile), heads = (float)p.pool.Hkv;
+        const float start = kStart[at][type][dims], key = kKey[at][type][dims], gain = kAtOnce[at][type][dims];
         const float record = 4.f * (float)paged_record_floats(rows, D);
         float last = 0.f;
         for (int n = 1; n <= 512; n = n < 8 ? n + 1 : n + n / 4) {
@@ -105,11 +105,13 @@ int64_t paged_plan(PagedAttnParams& p, const int64_t* keys, int cus) {
             last = len;
             float parts = 0.f;
             for (int b = 0; b < p.B; ++b) parts += std::max(1.f, up(rounds[b] * inv));
-            const float wgs = parts * units;
+            const float wgs = parts * heads * n_rb;
             if (n > 1 && wgs * record > (float)most_bytes) break;
+            // Row blocks of a (part, KV head) are on one XCD of 8.
+            const float on_cu = n_rb > 1.f ? up(up(parts * heads / 8.f) * n_rb * 8.f / (float)cus) : up(wgs / (float)cus);
             const float one = start + key * len * (float)step;
-            const float mean = start + key * total * units / wgs * (float)step;
-            const float share = up(wgs / (float)cus) * mean / kAtOnce[at][type];
+            const float mean = start + key * total * heads * n_rb / wgs * (float)step;
+            const float share = on_cu * mean / gain;
             float time = joined(one, share, memory);
             int combine = 0;
             if (n > 1) {
