@@ -225,7 +225,9 @@ def _native_calls(l):
         qk_norm_rope=call(mod.qk_norm_rope, "nne_qk_norm_rope"),
         paged_append=call(mod.paged_append, "nne_paged_append"),
         paged_attention=call(mod.paged_attention, "nne_paged_attention"),
-        paged_commit=call(mod.paged_commit, "nne_paged_commit"))
+        paged_commit=call(mod.paged_commit, "nne_paged_commit"),
+        qk_norm_rope_t=call(mod.qk_norm_rope_t, "nne_qk_norm_rope"),
+        paged_append_t=call(mod.paged_append_t, "nne_paged_append"))
 
 
 def _native():
@@ -762,16 +764,17 @@ def qkv_rope(x, w_packed, bq, bk, bv, rope, pos_dev, pos_host, num_heads, num_kv
     return q_out, k_out, v_out
 
 
-_torch = None
+_torch = _f32 = _i32 = None
 
 
 def _check_f32(index, *ts):
     """float32 tensors on GPU ``index``, and that is the current one (whose streams
     the calls run on).  (The checks of a small call's tensors: a device object and
     an import statement cost more than the rest of them.)"""
-    global _torch
+    global _torch, _f32, _i32
     if _torch is None:
         import torch
+        _f32, _i32 = torch.float32, torch.int32
         _torch = torch
     f32 = _torch.float32
     for t in ts:
@@ -893,6 +896,8 @@ def _rope_args(rope, index):
     if rope is None:
         return _NO_ROPE
     cos, sin = rope.cos, rope.sin
+    if cos.dtype is not _torch.float32 or sin.dtype is not _torch.float32:
+        raise InvalidArgument("Invalid configuration or argument: rotary tables of %s" % cos.dtype)
     if cos.get_device() != index or sin.get_device() != index:
         raise InvalidArgument("Invalid configuration or argument: the rotary tables are on %s, not on "
                               "GPU %d" % (cos.device, index))
@@ -906,6 +911,18 @@ def _check_out(out, shape, index):
                             % (list(shape), list(out.shape)))
 
 
+# qk_norm_rope and append hand their tensors to the native call first, which reads and
+# checks them (csrc/pycall.cpp); where it does not take them (None), the checks here tell
+# why, or make the call.
+
+def _rope_tensors(rope):
+    return _NO_ROPE if rope is None else (rope.cos, rope.sin, rope.max_seq_len, rope.head_dim)
+
+
+def _current(index):
+    return _f32 is not None and index >= 0 and _torch._C._cuda_getDevice() == index
+
+
 def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6, draft=None,
                  q_out=None, k_out=None, stream=None):
     """Per-head norm and rotation of queries and keys in one pass: each head x of
@@ -916,7 +933,24 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope, start_dev, start_host, eps=1e-6
     rope=None: no rotation; eps=None: no norm, the rotation alone (no weights);
     k=None: q alone.  Returns (q_out, k_out): new tensors in the inputs' order of dims
     by default, or the given ones (q and k themselves are fine)."""
-    qs, index = q.shape, q.get_device()
+    index = q.get_device()
+    if _current(index) and (draft is None or q.dim() == 4):
+        depths = _NO_PAIR
+        if draft is not None and rope is not None:
+            draft._check(q.shape[0], q.shape[2], index)
+            depths = draft._depths
+        qo = _new_like(q, stream) if q_out is None else q_out
+        ko = _new_like(k, stream) if k_out is None and k is not None else k_out
+        start = (None, None) if rope is None else (start_dev, start_host)
+        rc = _native().qk_norm_rope_t(
+            _f32, index, _i32, q, qo, k, ko, q_weight, k_weight, eps is not None,
+            0.0 if eps is None else eps, *_rope_tensors(rope), *start, *depths,
+            _stream_on(index, stream))
+        if rc == 0:
+            return qo, ko
+        if rc is not None:
+            check(rc)
+    qs = q.shape
     if k is None or q_weight is None or k_weight is None:
         _check_f32(index, *[t for t in (q, k, q_weight, k_weight) if t is not None])
     else:
@@ -1205,6 +1239,18 @@ class PagedKVCache:
         positions (``rope``: a RotaryEmbedding; None: as they are)."""
         self._check_layer(layer_idx)
         index = self._index
+        if _current(index) and (draft is None or k_new.dim() == 4):
+            counts = depths = _NO_PAIR
+            if draft is not None:
+                draft._check(k_new.shape[0], k_new.shape[2], index)
+                counts, depths = draft._counts, draft._depths
+            rc = _native().paged_append_t(
+                _f32, index, self._addr[layer_idx][0], k_new, v_new, *counts, *depths,
+                *_rope_tensors(rope), _stream_on(index, stream))
+            if rc == 0:
+                return
+            if rc is not None:
+                check(rc)
         _check_f32(index, k_new, v_new)
         shape = k_new.shape
         if len(shape) != 4:

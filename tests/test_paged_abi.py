@@ -348,10 +348,51 @@ def test_draft_trees_refuse(nne):
         tree._check(2, 4, -1)
 
 
-@pytest.mark.parametrize("name", ["qk_norm_rope", "paged_append", "paged_attention", "paged_commit"])
+@pytest.mark.parametrize("name", ["qk_norm_rope", "paged_append", "paged_attention", "paged_commit",
+                                  "qk_norm_rope_t", "paged_append_t"])
 def test_malformed_native_calls_raise(nne, name):
     call = getattr(nne._native(), name)
     with pytest.raises(TypeError):
         call()
-    with pytest.raises(TypeError):
+    with pytest.raises((TypeError, AttributeError)):
         call(*[object()] * 3)
+    with pytest.raises(TypeError):
+        call(*[None] * 40)
+
+
+def test_native_calls_on_tensors(nne):
+    """The calls that read tensors themselves: None for a tensor that does not fit, else
+    the ABI's answer (index -1: CPU tensors, which the ABI's checks refuse or do not reach)."""
+    import torch
+    f32, i32 = torch.float32, torch.int32
+    native = nne._native()
+    cache = Cache(nne)
+    addr = ctypes.addressof(cache.c)
+    k, q = torch.zeros(2, 2, 30, 16), torch.zeros(2, 4, 30, 16)
+
+    def append(k, v, addr=addr, index=-1):
+        return native.paged_append_t(f32, index, addr, k, v, None, None, None, None, None, None, 0, 0, 0)
+
+    assert append(k, k) == nne.NNE_ECAPACITY                  # 30 rows behind 5 and 9 of 32
+    for bad in (k.double(), k[0], k[:1], k[:, :1], k[..., :8], k.numpy(), torch.zeros(1, 2, 2, 30, 16)):
+        assert append(bad, k) is None and append(k, bad) is None
+    assert append(k, k, index=0) is None and append(k, k, addr=0) is None
+    cos = torch.zeros(8, 16)
+    start, host = torch.zeros(2, dtype=i32), np.array([0, 7], np.int32)
+
+    def norm(q=q, qo=q, k=k, ko=k, qw=None, kw=None, cos=cos, start=start, host=host, d=16):
+        return native.qk_norm_rope_t(f32, -1, i32, q, qo, k, ko, qw, kw, True, 1e-6, cos, cos, 8, d, start, host,
+                                     None, None, 0)
+
+    assert norm() == nne.NNE_EINVAL                           # rows 7..36 of 8
+    assert b"exceeds RoPE max_seq_len" in nne.lib().nne_last_error()
+    assert norm(d=8) == nne.NNE_ESHAPE
+    assert norm(k=None, ko=None) == nne.NNE_EINVAL
+    w = torch.ones(16)
+    assert norm(qw=w, kw=w) == nne.NNE_EINVAL
+    for bad in (dict(q=q.double()), dict(q=q[0]), dict(qo=q[:1]), dict(k=None), dict(ko=None), dict(ko=q),
+                dict(qw=torch.ones(8)), dict(kw=torch.ones(32)[::2]), dict(qw=w.double()), dict(kw=w[None]),
+                dict(cos=cos.double()), dict(start=start.long()), dict(start=start[:1]), dict(start=None),
+                dict(start=torch.zeros(4, dtype=i32)[::2]), dict(host=None), dict(host=host[:1]),
+                dict(host=host.astype(np.int64)), dict(host=[0, 7]), dict(host=np.zeros(4, np.int32)[::2])):
+        assert norm(**bad) is None, bad
