@@ -530,3 +530,91 @@ def test_python_calls_refuse(nne, cuda):
         cache.set_table([[0, 1], [0, 2]])
         cache.append(0, x, x)
     assert list(cache.lens_host) == [0, 0] and not cache.k.any() and not cache.v.any()
+
+
+def test_replayed_tokens(nne, cuda):
+    """A captured decode step -- norm and rotation, append, attention, commit of one -- is
+    the eager one: the same rows in the pools, replay after replay."""
+    import torch
+    rng = np.random.default_rng(71)
+    b, hq, hkv, d, page = 2, 6, 2, 64, 16
+    pages = P.Pages(rng, b, hkv, d, page, [510, 33], 12)
+    caches = [pages.cache(nne, cuda) for _ in range(2)]
+    rope = nne.RotaryEmbedding(d, 1024, device=cuda)
+    w = [_up(1 + rng.standard_normal(d, dtype=np.float32) / 8, cuda) for _ in range(2)]
+    x = [torch.zeros(b, 1, h, d, device=cuda).transpose(1, 2) for h in (hq, hkv, hkv)]
+    norms = [torch.zeros(b, h, 1, d, device=cuda) for h in (hq, hkv)]
+    out = torch.zeros(b, hq, 1, d, device=cuda)
+
+    def step(cache, q_out, k_out, o):
+        q, k = nne.qk_norm_rope(x[0], x[1], *w, rope, cache.lens_dev, cache.lens_host, q_out=q_out, k_out=k_out)
+        cache.append(0, k, x[2])
+        cache.attend(0, q, out=o)
+        cache.commit(1)
+        return q
+
+    def fill():
+        for a in x:
+            a.copy_(_up(rng.standard_normal(tuple(a.shape), dtype=np.float32), cuda))
+        torch.cuda.synchronize()
+
+    lens = pages.lens.copy()
+    fill()
+    step(caches[0], *norms, out)
+    caches[0].set_lengths(lens)                        # the warm-up's token does not count
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(caches[0], *norms, out)
+    for turn in range(6):
+        fill()
+        out.fill_(7.0)
+        graph.replay()
+        q = step(caches[1], None, None, None if turn % 2 else torch.zeros_like(out))
+        torch.cuda.synchronize()
+        assert torch.equal(norms[0], q), turn
+        k, v = P.host(caches[1].k), P.host(caches[1].v)
+        rows = [np.concatenate([pages.table[i, :(n + turn + page) // page] for i, n in enumerate(lens)])]
+        for pool, want in ((caches[0].k, k), (caches[0].v, v)):
+            assert np.array_equal(P.host(pool)[0][rows[0]], want[0][rows[0]]), turn
+        _check_attend(out.cpu().numpy(), q.cpu().numpy(), k[0], v[0], pages.table, page, lens + turn, [1] * b, None,
+                      "replay %d" % turn)
+        assert caches[0].lens_dev.tolist() == caches[1].lens_dev.tolist() == (lens + turn + 1).tolist()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pages_outside_the_pool(nne, cuda, dtype):
+    """Without the host's table the device's own bounds hold: a row whose page lies outside
+    is not written, and attention leaves it out."""
+    import torch
+    lib = nne.lib()
+    rng = np.random.default_rng(72)
+    b, hq, hkv, d, page, t = 2, 4, 2, 64, 8, 5
+    pages = P.Pages(rng, b, hkv, d, page, [40, 21], t, dtype=dtype)
+    cache = pages.cache(nne, cuda)
+    bad = pages.table.copy()
+    bad[0, 1], bad[0, 3], bad[1, 0] = -1, pages.n_pages, 2 ** 31 - 1     # of counted rows
+    bad[1, 3] = -5                                                       # rows 24, 25 of the new ones
+    cache.table_dev.copy_(_up(bad, cuda))
+    q, k, v = (rng.standard_normal((b, h, t, d), dtype=np.float32) for h in (hq, hkv, hkv))
+    dev = [_up(a, cuda) for a in (q, k, v)]
+    out = torch.full((b, hq, t, d), 7.0, device=cuda)
+    addr, stream = cache._addr[0][1], torch.cuda.current_stream().cuda_stream
+    nne.check(lib.nne_paged_append(addr, dev[1].data_ptr(), None, dev[2].data_ptr(), None, t, None, None, None, None,
+                                   None, None, 0, 0, stream))
+    nne.check(lib.nne_paged_attention(addr, dev[0].data_ptr(), None, out.data_ptr(), None, hq, t, None, None, None,
+                                      None, 0, 0.0, None, stream))
+    torch.cuda.synchronize()
+    for i in range(b):
+        for n in range(t):
+            r = int(pages.lens[i]) + n
+            if 0 <= bad[i, r // page] < pages.n_pages:
+                pages.put(pages.k, i, r, k[i, :, n])
+                pages.put(pages.v, i, r, v[i, :, n])
+    assert np.array_equal(P.host(cache.k), pages.k) and np.array_equal(P.host(cache.v), pages.v)
+    for i in range(b):
+        n = int(pages.lens[i]) + t
+        there = np.array([0 <= bad[i, r // page] < pages.n_pages for r in range(n)])
+        assert there.any() and not there.all()
+        want, bound = P.attention64(q[i], pages.rows(pages.k, i, n), pages.rows(pages.v, i, n),
+                                    P.visible(n - t, t, None) & there, 1 / math.sqrt(d))
+        _close(out.cpu().numpy()[i], want, bound, "sequence %d" % i)
