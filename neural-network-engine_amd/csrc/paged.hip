@@ -28,9 +28,10 @@ __device__ __forceinline__ vf4 load_row4(const float* row, int64_t sd, int i, bo
 }
 
 // Rotates dims i..i+3 (a) and i + d/2.. (b) of a row with the table row.
+template <bool VEC>
 __device__ __forceinline__ void rotate4(vf4& a, vf4& b, const float* c, const float* s, int i, int half) {
-    const vf4 c0 = *reinterpret_cast<const vf4*>(c + i), s0 = *reinterpret_cast<const vf4*>(s + i);
-    const vf4 c1 = *reinterpret_cast<const vf4*>(c + i + half), s1 = *reinterpret_cast<const vf4*>(s + i + half);
+    const vf4 c0 = load_row4(c, 1, i, VEC), s0 = load_row4(s, 1, i, VEC);
+    const vf4 c1 = load_row4(c, 1, i + half, VEC), s1 = load_row4(s, 1, i + half, VEC);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float x = a[j], y = b[j];
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendPara
             int pos = len + (p.depths ? p.depths[(int64_t)b * p.T + t] : t);
             pos = pos < 0 ? 0 : pos >= p.max_seq_len ? p.max_seq_len - 1 : pos;
             const int64_t at = (int64_t)pos * p.pool.d;
-            rotate4(k0, k1, p.cos + at, p.sin + at, i, half);
+            rotate4<true>(k0, k1, p.cos + at, p.sin + at, i, half);
         }
         const int64_t at = (int64_t)row * p.pool.d + i;
         store_row4<BF16>(p.pool.k, at, k0);
@@ -185,8 +186,9 @@ __device__ __forceinline__ int64_t norm_table_row(const NormRopeParams& p, int b
 // exchanges.  A head is read once and written once, and the memory bounds a long
 // launch.  STREAM: the outputs are more than the L2s hold, and pass them by.  4
 // sequences of 1999 tokens of 32 + 8 heads of 64 dims, 164 MB: 29 us (5.6 TB/s),
-// 33 us without; 32 single tokens of 32 + 8 heads of 128 dims: 3.7 us.
-template <int LPR, bool STREAM>
+// 33 us without; 32 single tokens of 32 + 8 heads of 128 dims: 3.7 us.  VEC: every row
+// is 16-byte vectors (the long launch at other addresses: 57 us).
+template <int LPR, bool STREAM, bool VEC>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NormRopeParams p) {
     const int heads = p.H[0] + p.H[1], half = p.d / 2;
     const uint32_t n = (uint32_t)p.B * p.T * heads;           // (the host keeps this in 31 bits)
@@ -202,8 +204,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NormRopeParams 
         const float* row = x.p + b * x.sb + h * x.sh + t * x.st;
         vf4 y0 = vf4{0.f, 0.f, 0.f, 0.f}, y1 = y0;
         if (in) {
-            y0 = *reinterpret_cast<const vf4*>(row + i);
-            y1 = *reinterpret_cast<const vf4*>(row + i + half);
+            y0 = load_row4(row, x.sd, i, VEC);
+            y1 = load_row4(row, x.sd, i + half, VEC);
         }
         const int64_t tab = p.cos ? norm_table_row(p, b, t) : 0;
         float sum = 0.f;
@@ -215,12 +217,18 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NormRopeParams 
         if (!in) continue;
         const float* w = which ? p.w[1] : p.w[0];
         const vf4 one = vf4{1.f, 1.f, 1.f, 1.f};
-        y0 = y0 * scale * (w ? *reinterpret_cast<const vf4*>(w + i) : one);
-        y1 = y1 * scale * (w ? *reinterpret_cast<const vf4*>(w + i + half) : one);
-        if (p.cos) rotate4(y0, y1, p.cos + tab, p.sin + tab, i, half);
+        y0 = y0 * scale * (w ? load_row4(w, 1, i, VEC) : one);
+        y1 = y1 * scale * (w ? load_row4(w, 1, i + half, VEC) : one);
+        if (p.cos) rotate4<VEC>(y0, y1, p.cos + tab, p.sin + tab, i, half);
         const OutView4 o = which ? p.o[1] : p.o[0];
         float* out = o.p + b * o.sb + h * o.sh + t * o.st;
-        if constexpr (STREAM) {
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                out[(i + j) * o.sd] = y0[j];
+                out[(i + half + j) * o.sd] = y1[j];
+            }
+        } else if constexpr (STREAM) {
             __builtin_nontemporal_store(y0, reinterpret_cast<vf4*>(out + i));
             __builtin_nontemporal_store(y1, reinterpret_cast<vf4*>(out + i + half));
         } else {
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NormRopeParams 
     }
 }
 
-// Any even d and any strides: a wave per head, which reads it twice.
+// Any other even d: a wave per head, which reads it twice.
 __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(const NormRopeParams p) {
     const int heads = p.H[0] + p.H[1], half = p.d / 2, lane = threadIdx.x & 63;
     const int64_t n = (int64_t)p.B * p.T * heads;
@@ -309,7 +317,7 @@ hipError_t launch_qk_norm_rope(const NormRopeParams& p, hipStream_t stream) {
     const int64_t n = (int64_t)p.B * p.T * (p.H[0] + p.H[1]);
     if (n <= 0) return hipSuccess;
     const int64_t most = 1 << 20;
-    if (!p.vec || n > INT32_MAX) {
+    if (p.d % 8 != 0 || p.d > 512 || n > INT32_MAX) {
         hipLaunchKernelGGL(qk_norm_rope_any_kernel, dim3(grid_for(n * 64, most)), dim3(256), 0, stream, p);
         return hipGetLastError();
     }
@@ -317,8 +325,9 @@ hipError_t launch_qk_norm_rope(const NormRopeParams& p, hipStream_t stream) {
     const auto launch = [&](auto lpr) {
         constexpr int LPR = decltype(lpr)::value;
         const dim3 grid(grid_for(n * LPR, most));
-        if (streams) hipLaunchKernelGGL((qk_norm_rope_kernel<LPR, true>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((qk_norm_rope_kernel<LPR, false>), grid, dim3(256), 0, stream, p);
+        if (!p.vec) hipLaunchKernelGGL((qk_norm_rope_kernel<LPR, false, false>), grid, dim3(256), 0, stream, p);
+        else if (streams) hipLaunchKernelGGL((qk_norm_rope_kernel<LPR, true, true>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((qk_norm_rope_kernel<LPR, false, true>), grid, dim3(256), 0, stream, p);
     };
     if (p.d <= 64) launch(std::integral_constant<int, 8>());
     else if (p.d <= 128) launch(std::integral_constant<int, 16>());

@@ -117,7 +117,7 @@ struct NormRopeParams {
     const float *cos, *sin;    // null: no rotation
     int max_seq_len;
     const int32_t *start, *depths;
-    int vec;
+    int vec;                   // rows, weights and tables are 16-byte vectors
 };
 
 }  // namespace nne

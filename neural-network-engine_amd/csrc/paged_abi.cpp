@@ -260,7 +260,7 @@ int nne_qk_norm_rope(const float* q, const int64_t q_shape[4], const int64_t q_s
     p.max_seq_len = (int)max_seq_len;
     p.start = start_dev;
     p.depths = depths_dev;
-    p.vec = d % 8 == 0 && d <= 512 && vec_view(q, qs.v) && vec_view(q_out, qo.v) &&
+    p.vec = vec_view(q, qs.v) && vec_view(q_out, qo.v) &&
             (Hk == 0 || (vec_view(k, ks.v) && vec_view(k_out, ko.v))) && aligned16(q_weight) &&
             aligned16(k_weight) && aligned16(cos_table) && aligned16(sin_table);
     const hipError_t e = nne::launch_qk_norm_rope(p, static_cast<hipStream_t>(stream));
