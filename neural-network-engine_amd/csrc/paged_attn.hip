@@ -29,7 +29,7 @@
 // 128 dims, take 107 us on an f32 pool (606 MB, 5.7 TB/s; a large copy runs at 4.9)
 // and 59 on a bf16 one (5.1 TB/s); 5 tokens of 16 of them 37 us (4.1 TB/s).  Trees of
 // many rows are bound by the matrix cores and what they wait for: 64 tokens of 8
-// sequences of 1024-4096 keys take 80 us, 825 TFLOP/s of bf16 products (30 % of the
+// sequences of 1024-4096 keys take 80 us, 825 TFLOP/s of bf16 products (31 % of the
 // MFMAs' cycles; a large library product of that type reaches 1146).  Two waves per
 // SIMD is what the registers of 32 rows allow.  Bringing K to LDS in whole lines
 // first was level (79 us), 128 rows per workgroup with K and V in LDS slower (99 us).
