@@ -618,3 +618,30 @@ def test_pages_outside_the_pool(nne, cuda, dtype):
         want, bound = P.attention64(q[i], pages.rows(pages.k, i, n), pages.rows(pages.v, i, n),
                                     P.visible(n - t, t, None) & there, 1 / math.sqrt(d))
         _close(out.cpu().numpy()[i], want, bound, "sequence %d" % i)
+
+
+def test_replay_after_the_workspace_grew(nne, cuda):
+    """A captured call keeps its records where they were when the workspace grows."""
+    import torch
+    rng = np.random.default_rng(73)
+    pages = P.Pages(rng, 2, 2, 64, 16, [2500, 900], 64)
+    cache = pages.cache(nne, cuda)
+    q = [rng.standard_normal((2, 4, t, 64), dtype=np.float32) for t in (1, 64)]
+    dev = [_up(a, cuda) for a in q]
+    out = torch.zeros_like(dev[0])
+    cache.attend(0, dev[0], out=out)
+    torch.cuda.synchronize()
+    before = cache._ws.records.data_ptr()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(0, dev[0], out=out)
+    for turn in range(3):
+        big = cache.attend(0, dev[1])
+        assert cache._ws.records.data_ptr() != before
+        filler = [torch.full((1 << 20,), float("nan"), device=cuda) for _ in range(8)]   # (what was freed)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_attend(out.cpu().numpy(), q[0], pages.k[0], pages.v[0], pages.table, 16, pages.lens, [1, 1], None, "replay")
+        _check_attend(big.cpu().numpy(), q[1], pages.k[0], pages.v[0], pages.table, 16, pages.lens, [64, 64], None, "eager")
+        assert all(torch.isnan(f).all() for f in filler)
